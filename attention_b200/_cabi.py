@@ -30,6 +30,13 @@ SIGNATURES = {
     "gqa_b200_prefill": (c_int, [_P] * 6 + [c_int] * 7 + [c_float, c_int, c_int, _P]),
     "gqa_b200_prefill_tc_status": (c_int, [c_int]),
     "gqa_b200_kv_append": (c_int, [_P] * 6 + [c_int] * 4 + [c_int64, c_int, c_int, _P]),
+    "gqa_b200_qk_norm_rope": (c_int, [_P] * 13 + [c_int] * 8 + [c_int64, _P, c_float, c_int, c_int64,
+                                                               c_int, c_int, _P]),
+    "gqa_b200_tree_workspace_bytes": (c_size_t, [c_int] * 7),
+    "gqa_b200_tree_decode": (c_int, [_P] * 8 + [c_int] * 6 + [c_int64, c_int, c_int, c_float, c_int, _P,
+                                                              c_size_t, _P]),
+    "gqa_b200_kv_compact": (c_int, [_P] * 5 + [c_int] * 5 + [c_int64, c_int, c_int, _P]),
+    "gqa_b200_kv_copy_pages": (c_int, [_P] * 4 + [c_int] * 4 + [c_int64, c_int, _P]),
     # include/mla_decode_b200.h
     "mla_b200_project": (c_int, [_P] * 3 + [c_int, c_int64] + [c_int] * 4 + [_P]),
     "mla_b200_latent_kv_write": (c_int, [_P] * 4 + [c_int64, c_int, c_int, c_int, _P]),

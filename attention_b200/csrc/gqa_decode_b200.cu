@@ -446,6 +446,10 @@ const char* gqa_b200_strerror(int code) {
         case GQA_B200_ERR_STATIC_LIMIT:
             return "shape needs more scratch than gqa_b200_decode_static's built-in "
                    "GQA_B200_STATIC_SCRATCH_BYTES; use gqa_b200_decode with a caller workspace";
+        case GQA_B200_ERR_TREE_TOKENS: return "drafted tokens per sequence must be in [1, 64]";
+        case GQA_B200_ERR_ROTATION:
+            return "rot_dim must be even and in [0, head_dim], max_position in [0, 2^31)";
+        case GQA_B200_ERR_COMPACT_ROWS: return "kv_compact moves at most 1024 rows per sequence";
         case MLA_B200_ERR_SHAPE: return "MLA: a width, head count, tq or nk is not positive";
         case MLA_B200_ERR_LATENT_DIM: return "MLA: supported latent width dc is [1, 512]";
         default: break;

@@ -1,0 +1,349 @@
+// Host side of the speculative-step entry points declared in include/gqa_decode_b200.h: norm and
+// rotation (into pages), tree attention, compaction of an accepted path, page copies.  Argument
+// checks, the cut of the work and the launches.  No allocation, no synchronisation.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <cstdlib>
+#include <limits>
+#include <mutex>
+
+#include "../../include/gqa_decode_b200.h"
+#include "gqa_tree_simt.cuh"
+#include "kv_pages.cuh"
+#include "qk_norm_rope.cuh"
+
+namespace gqa_b200 {
+namespace {
+
+constexpr int kSms = 148;                    // the cut of the work is for a B200, whatever runs it
+constexpr int kTreeSimtCtasPerSm = 3;
+constexpr long long kIntMax = 0x7fffffffll;
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+inline int elem_size(int dtype) { return dtype == GQA_B200_F32 ? 4 : 2; }
+inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+inline bool known_dtype(int dtype) {
+    return dtype == GQA_B200_F32 || dtype == GQA_B200_F16 || dtype == GQA_B200_BF16;
+}
+
+std::mutex g_mutex;                          // guards the per-device caches of this file
+
+bool pdl_on() {
+    static const bool on = [] {
+        const char* e = std::getenv("GQA_B200_NO_PDL");
+        return !(e && e[0] == '1');
+    }();
+    return on;
+}
+
+// Launch with programmatic stream serialization: the kernel may start while its predecessor in the
+// stream drains; every kernel launched this way executes griddepcontrol.wait before its first
+// global access.  GQA_B200_NO_PDL=1 in the environment turns it off.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pdl(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_on() ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
+
+// Raises a kernel's dynamic shared-memory limit once per device.
+cudaError_t allow_smem(const void* kernel, size_t smem) {
+    struct Entry { const void* kernel; int dev; };
+    static Entry done[256];
+    static int n_done = 0;
+    if (smem <= 48 * 1024) return cudaSuccess;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    std::lock_guard<std::mutex> lock(g_mutex);
+    for (int i = 0; i < n_done; ++i)
+        if (done[i].kernel == kernel && done[i].dev == dev) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess && n_done < 256) done[n_done++] = Entry{kernel, dev};
+    return e;
+}
+
+// ---------------------------------------------------------------------------
+// tree attention
+// ---------------------------------------------------------------------------
+// Number of runs the tiles are cut into for `units` CTAs per run on `slots` resident CTAs: as many
+// as fill the GPU once, or up to four times if that leaves fewer CTAs idle in the last round (a
+// single round of 4 runs x 32 kv heads would leave 20 of 148 SMs without work; two rounds of 288
+// CTAs leave 8 of 296).
+int tree_run_count(long long units, long long slots, long long cap_tiles) {
+    long long best = 1;
+    double best_fill = 0.0;
+    for (int rounds = 1; rounds <= 4; ++rounds) {
+        const long long n = slots * rounds / units;
+        if (n < 1) continue;
+        const double fill = (double)(n * units) / (double)(slots * rounds);
+        if (fill > best_fill + 0.03) { best_fill = fill; best = n; }
+    }
+    return (int)std::max(1ll, std::min(best, cap_tiles));
+}
+
+int tree_simt_rows(int rows) { return rows <= 8 ? 8 : rows <= 16 ? 16 : 32; }
+
+struct TreePlan {
+    int row_block, row_blocks, n_runs;
+    long long units;
+};
+TreePlan tree_plan(int batch, int tokens, int q_heads, int kv_heads, long long cap_tokens, int row_block, int ctas_per_sm) {
+    TreePlan t;
+    const long long rows = (long long)tokens * (q_heads / kv_heads);
+    t.row_block = row_block;
+    t.row_blocks = (int)((rows + row_block - 1) / row_block);
+    t.units = (long long)kv_heads * t.row_blocks;
+    const long long cap_tiles = (long long)batch * ((cap_tokens + kTreeTile - 1) / kTreeTile);
+    t.n_runs = tree_run_count(t.units, (long long)kSms * ctas_per_sm, cap_tiles);
+    return t;
+}
+TreePlan tree_plan_simt(int batch, int tokens, int q_heads, int kv_heads, long long cap_tokens) {
+    return tree_plan(batch, tokens, q_heads, kv_heads, cap_tokens, tree_simt_rows(tokens * (q_heads / kv_heads)),
+                     kTreeSimtCtasPerSm);
+}
+
+struct TreeScratch {
+    size_t info, ml, acc, total;
+};
+TreeScratch tree_scratch(const TreePlan& t, int tokens, int q_heads, int head_dim) {
+    TreeScratch s;
+    const size_t rows = t.n_runs > 1 ? 2 * (size_t)t.n_runs * tokens * q_heads : 0;
+    s.info = 0;
+    s.ml = align_up((size_t)(t.n_runs + 1) * sizeof(int4), 256);
+    s.acc = s.ml + align_up(rows * sizeof(float2), 256);
+    s.total = s.acc + align_up(rows * head_dim * sizeof(float), 256);
+    return s;
+}
+
+inline long long cap_tokens_of(int max_pages, int block_size) {
+    return std::min((long long)max_pages * block_size, kIntMax - kTreeTile);
+}
+
+template <typename T, int RB, int DC>
+cudaError_t launch_tree_simt(const TreeParams& p, const TreePlan& t, bool vec, cudaStream_t stream) {
+    constexpr size_t smem = TreeSimtGeom<RB, DC>::kSmemBytes;
+    auto kernel = gqa_tree_simt_kernel<T, RB, DC>;
+    const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), smem);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(kernel, dim3((unsigned)(t.n_runs * t.units)), kTreeSimtThreads, smem, stream, p, (int)vec);
+}
+template <typename T, int RB>
+cudaError_t launch_tree_simt_dim(const TreeParams& p, const TreePlan& t, bool vec, cudaStream_t stream) {
+    if (p.head_dim <= 64) return launch_tree_simt<T, RB, 64>(p, t, vec, stream);
+    if (p.head_dim <= 128) return launch_tree_simt<T, RB, 128>(p, t, vec, stream);
+    return launch_tree_simt<T, RB, 256>(p, t, vec, stream);
+}
+template <typename T>
+cudaError_t launch_tree(const TreeParams& p, const TreePlan& t, bool vec, cudaStream_t stream) {
+    cudaError_t e;
+    switch (t.row_block) {
+        case 8:  e = launch_tree_simt_dim<T, 8>(p, t, vec, stream); break;
+        case 16: e = launch_tree_simt_dim<T, 16>(p, t, vec, stream); break;
+        default: e = launch_tree_simt_dim<T, 32>(p, t, vec, stream); break;
+    }
+    if (e != cudaSuccess || t.n_runs == 1) return e;
+    const int rows = p.rows * p.kv_heads;
+    const int by = std::min((rows + kTreeMergeWarps - 1) / kTreeMergeWarps, 65535);
+    return launch_pdl(gqa_tree_merge_kernel<T>, dim3((unsigned)(t.n_runs - 1), (unsigned)by), kTreeMergeWarps * 32, 0,
+                      stream, p);
+}
+
+// ---------------------------------------------------------------------------
+// norm and rotation
+// ---------------------------------------------------------------------------
+template <typename T>
+cudaError_t launch_rope(const RopeParams& p, cudaStream_t stream) {
+    const int heads = p.q_heads + p.kv_heads * (p.append ? 2 : 1);
+    const long long rows = p.n_tokens * heads;
+    const long long grid = (rows + kRopeWarps - 1) / kRopeWarps;
+    if (grid > kIntMax) return cudaErrorInvalidValue;
+    qk_norm_rope_any_kernel<T><<<(unsigned)grid, kRopeWarps * 32, 0, stream>>>(p);
+    return cudaGetLastError();
+}
+
+}  // namespace
+}  // namespace gqa_b200
+
+using namespace gqa_b200;
+
+extern "C" {
+
+int gqa_b200_qk_norm_rope(const void* q, const void* k, const void* v, const void* q_weight, const void* k_weight,
+                          const float* cos_sin, const int32_t* positions, void* q_out, void* k_out, void* k_cache,
+                          void* v_cache, const int32_t* block_table, const int32_t* slots, int dtype, int weight_dtype,
+                          int batch, int tokens, int q_heads, int kv_heads, int head_dim, int rot_dim,
+                          int64_t max_position, const int64_t* strides, float eps, int interleaved, int64_t num_blocks,
+                          int block_size, int max_pages, void* stream) {
+    if (!known_dtype(dtype) || (weight_dtype != dtype && weight_dtype != GQA_B200_F32)) return GQA_B200_ERR_DTYPE;
+    if (batch < 0 || tokens < 0) return GQA_B200_ERR_BATCH;
+    if (q_heads <= 0 || kv_heads <= 0) return GQA_B200_ERR_HEADS;
+    if (head_dim <= 0 || head_dim > 256) return GQA_B200_ERR_HEAD_DIM;
+    if (rot_dim < 0 || rot_dim > head_dim || rot_dim % 2 != 0 || max_position < 0 || max_position > kIntMax)
+        return GQA_B200_ERR_ROTATION;
+    if (!(std::isfinite(eps) && eps >= 0.f)) return GQA_B200_ERR_SCALE;
+    if (!strides || (!q_weight) != (!k_weight)) return GQA_B200_ERR_NULL_POINTER;
+    if (batch == 0 || tokens == 0) return GQA_B200_OK;
+    const bool append = k_cache != nullptr;
+    if (!q || !k || !q_out || !positions || (rot_dim > 0 && max_position > 0 && !cos_sin)) return GQA_B200_ERR_NULL_POINTER;
+    if (append) {
+        if (num_blocks <= 0 || block_size <= 0) return GQA_B200_ERR_CACHE_SHAPE;
+        if (max_pages <= 0) return GQA_B200_ERR_MAX_PAGES;
+        if (num_blocks > kIntMax) return GQA_B200_ERR_INT32_RANGE;
+        if (!v || !v_cache || !block_table || !slots) return GQA_B200_ERR_NULL_POINTER;
+    } else if (!k_out) {
+        return GQA_B200_ERR_NULL_POINTER;
+    }
+    RopeParams p{};
+    p.q = q; p.k = k; p.v = v; p.q_weight = q_weight; p.k_weight = k_weight; p.cos_sin = cos_sin;
+    p.positions = positions; p.slots = slots; p.table = block_table;
+    p.q_out = q_out; p.k_out = k_out; p.k_cache = k_cache; p.v_cache = v_cache;
+    p.q_sb = strides[0]; p.q_st = strides[1]; p.q_sh = strides[2];
+    p.k_sb = strides[3]; p.k_st = strides[4]; p.k_sh = strides[5];
+    p.v_sb = strides[6]; p.v_st = strides[7]; p.v_sh = strides[8];
+    p.num_blocks = num_blocks;
+    p.cap_tokens = append ? std::min((long long)max_pages * block_size, kIntMax) : 0;
+    p.n_tokens = (long long)batch * tokens;
+    p.tokens = tokens; p.q_heads = q_heads; p.kv_heads = kv_heads; p.head_dim = head_dim; p.rot_dim = rot_dim;
+    p.max_position = (int)max_position; p.block_size = block_size; p.max_pages = max_pages;
+    p.append = append ? 1 : 0; p.interleaved = interleaved ? 1 : 0; p.weight_f32 = weight_dtype == GQA_B200_F32;
+    p.eps = eps;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (dtype) {
+        case GQA_B200_F32: return (int)launch_rope<float>(p, s);
+        case GQA_B200_F16: return (int)launch_rope<__half>(p, s);
+        default:           return (int)launch_rope<__nv_bfloat16>(p, s);
+    }
+}
+
+size_t gqa_b200_tree_workspace_bytes(int batch, int tokens, int q_heads, int kv_heads, int head_dim, int block_size,
+                                     int max_pages) {
+    if (batch <= 0 || tokens <= 0 || tokens > kTreeMaxTokens || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads ||
+        head_dim <= 0 || head_dim > 256 || block_size <= 0 || max_pages <= 0)
+        return 0;
+    const long long cap = cap_tokens_of(max_pages, block_size);
+    return tree_scratch(tree_plan_simt(batch, tokens, q_heads, kv_heads, cap), tokens, q_heads, head_dim).total;
+}
+
+int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+                         const int32_t* context_lens, const int32_t* draft_lens, const int64_t* tree_mask, void* out,
+                         int dtype, int batch, int tokens, int q_heads, int kv_heads, int head_dim, int64_t num_blocks,
+                         int block_size, int max_pages, float scale, int kernel, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+    if (!known_dtype(dtype)) return GQA_B200_ERR_DTYPE;
+    if (batch < 0) return GQA_B200_ERR_BATCH;
+    if (tokens < 1 || tokens > kTreeMaxTokens) return GQA_B200_ERR_TREE_TOKENS;
+    if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads != 0) return GQA_B200_ERR_HEADS;
+    if (head_dim <= 0 || head_dim > 256) return GQA_B200_ERR_HEAD_DIM;
+    if (num_blocks <= 0 || block_size <= 0) return GQA_B200_ERR_CACHE_SHAPE;
+    if (max_pages <= 0) return GQA_B200_ERR_MAX_PAGES;
+    if (!(std::isfinite(scale) && scale > 0.f)) return GQA_B200_ERR_SCALE;
+    if (num_blocks > kIntMax || (long long)tokens * q_heads > 65535) return GQA_B200_ERR_INT32_RANGE;
+    if (kernel != GQA_B200_KERNEL_AUTO && kernel != GQA_B200_KERNEL_SIMT) return GQA_B200_ERR_KERNEL;
+    if (batch == 0) return GQA_B200_OK;
+    if (!q || !k_cache || !v_cache || !block_table || !context_lens || !out) return GQA_B200_ERR_NULL_POINTER;
+
+    const long long cap = cap_tokens_of(max_pages, block_size);
+    const TreePlan plan = tree_plan_simt(batch, tokens, q_heads, kv_heads, cap);
+    if (plan.n_runs * plan.units > kIntMax) return GQA_B200_ERR_INT32_RANGE;
+    const TreeScratch lay = tree_scratch(plan, tokens, q_heads, head_dim);
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < lay.total)
+        return GQA_B200_ERR_WORKSPACE;
+    char* ws = static_cast<char*>(workspace);
+    TreeParams p{};
+    p.q = q; p.k = k_cache; p.v = v_cache; p.out = out;
+    p.table = block_table; p.lens = context_lens; p.draft_lens = draft_lens;
+    p.mask = reinterpret_cast<const unsigned long long*>(tree_mask);
+    p.info = reinterpret_cast<int4*>(ws + lay.info);
+    p.part_ml = reinterpret_cast<float2*>(ws + lay.ml);
+    p.part_acc = reinterpret_cast<float*>(ws + lay.acc);
+    p.n_ranges = plan.n_runs;
+    p.batch = batch; p.tokens = tokens; p.q_heads = q_heads; p.kv_heads = kv_heads; p.group = q_heads / kv_heads;
+    p.head_dim = head_dim; p.rows = tokens * p.group; p.row_blocks = plan.row_blocks;
+    p.block_size = block_size; p.max_pages = max_pages; p.num_blocks = num_blocks;
+    p.bs_shift = -1;
+    for (int s = 0; s < 31; ++s)
+        if (block_size == 1 << s) p.bs_shift = s;
+    p.cap_tokens = (int)cap;
+    p.scale_log2 = scale * kLog2e;
+    const bool vec = head_dim * elem_size(dtype) % 16 == 0 && aligned16(q) && aligned16(k_cache) && aligned16(v_cache);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    switch (dtype) {
+        case GQA_B200_F32: return (int)launch_tree<float>(p, plan, vec, s);
+        case GQA_B200_F16: return (int)launch_tree<__half>(p, plan, vec, s);
+        default:           return (int)launch_tree<__nv_bfloat16>(p, plan, vec, s);
+    }
+}
+
+int gqa_b200_kv_compact(void* k_cache, void* v_cache, const int32_t* block_table, const int32_t* src_positions,
+                        const int32_t* dst_positions, int dtype, int batch, int n, int kv_heads, int head_dim,
+                        int64_t num_blocks, int block_size, int max_pages, void* stream) {
+    if (!known_dtype(dtype)) return GQA_B200_ERR_DTYPE;
+    if (batch < 0 || n < 0) return GQA_B200_ERR_BATCH;
+    if (n > kCompactMaxRows) return GQA_B200_ERR_COMPACT_ROWS;
+    if (kv_heads <= 0) return GQA_B200_ERR_HEADS;
+    if (head_dim <= 0) return GQA_B200_ERR_HEAD_DIM;
+    if (num_blocks <= 0 || block_size <= 0) return GQA_B200_ERR_CACHE_SHAPE;
+    if (max_pages <= 0) return GQA_B200_ERR_MAX_PAGES;
+    if (num_blocks > kIntMax) return GQA_B200_ERR_INT32_RANGE;
+    if (batch == 0 || n == 0) return GQA_B200_OK;
+    if (!k_cache || !v_cache || !block_table || !src_positions || !dst_positions) return GQA_B200_ERR_NULL_POINTER;
+    CompactParams p{};
+    p.k_cache = k_cache; p.v_cache = v_cache; p.table = block_table; p.src = src_positions; p.dst = dst_positions;
+    p.row_bytes = (long long)kv_heads * head_dim * elem_size(dtype);
+    p.num_blocks = num_blocks; p.cap_tokens = std::min((long long)max_pages * block_size, kIntMax);
+    p.n = n; p.block_size = block_size; p.max_pages = max_pages;
+    const int unit = p.row_bytes % 16 == 0 && aligned16(k_cache) && aligned16(v_cache) ? 16 : elem_size(dtype);
+    const long long units = p.row_bytes / unit;
+    const long long fit = (long long)kCompactThreads * kCompactItems / n;      // >= 1
+    p.slice = (int)std::min(units, fit);
+    const long long slices = (units + p.slice - 1) / p.slice;
+    if (slices > 65535) return GQA_B200_ERR_INT32_RANGE;
+    const dim3 grid((unsigned)batch, (unsigned)slices, 2);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (unit == 16) kv_compact_kernel<uint4><<<grid, kCompactThreads, 0, s>>>(p);
+    else if (unit == 4) kv_compact_kernel<uint32_t><<<grid, kCompactThreads, 0, s>>>(p);
+    else kv_compact_kernel<uint16_t><<<grid, kCompactThreads, 0, s>>>(p);
+    return (int)cudaGetLastError();
+}
+
+int gqa_b200_kv_copy_pages(void* k_cache, void* v_cache, const int32_t* src_pages, const int32_t* dst_pages, int dtype,
+                           int n, int kv_heads, int head_dim, int64_t num_blocks, int block_size, void* stream) {
+    if (!known_dtype(dtype)) return GQA_B200_ERR_DTYPE;
+    if (n < 0) return GQA_B200_ERR_BATCH;
+    if (kv_heads <= 0) return GQA_B200_ERR_HEADS;
+    if (head_dim <= 0) return GQA_B200_ERR_HEAD_DIM;
+    if (num_blocks <= 0 || block_size <= 0) return GQA_B200_ERR_CACHE_SHAPE;
+    if (num_blocks > kIntMax) return GQA_B200_ERR_INT32_RANGE;
+    if (n == 0) return GQA_B200_OK;
+    if (!k_cache || !v_cache || !src_pages || !dst_pages) return GQA_B200_ERR_NULL_POINTER;
+    const long long bytes = (long long)block_size * kv_heads * head_dim * elem_size(dtype);
+    const int unit = bytes % 16 == 0 && aligned16(k_cache) && aligned16(v_cache) ? 16 : elem_size(dtype);
+    PageCopyParams p{};
+    p.k_cache = k_cache; p.v_cache = v_cache; p.src = src_pages; p.dst = dst_pages;
+    p.page_units = bytes / unit;
+    p.num_blocks = num_blocks;
+    p.parts = (p.page_units + kPageCopyThreads * kPageCopyItems - 1) / (kPageCopyThreads * kPageCopyItems);
+    if (p.parts * n > kIntMax) return GQA_B200_ERR_INT32_RANGE;
+    const dim3 grid((unsigned)(p.parts * n), 2);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (unit == 16) kv_copy_pages_kernel<uint4><<<grid, kPageCopyThreads, 0, s>>>(p);
+    else if (unit == 4) kv_copy_pages_kernel<uint32_t><<<grid, kPageCopyThreads, 0, s>>>(p);
+    else kv_copy_pages_kernel<uint16_t><<<grid, kPageCopyThreads, 0, s>>>(p);
+    return (int)cudaGetLastError();
+}
+
+}  // extern "C"

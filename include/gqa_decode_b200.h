@@ -64,6 +64,9 @@ extern "C" {
 #define GQA_B200_ERR_CHUNK (-12)      /* chunk_tokens out of range              */
 #define GQA_B200_ERR_INT32_RANGE (-13)/* tensor sizes exceed int32 launch limits */
 #define GQA_B200_ERR_STATIC_LIMIT (-14) /* shape needs more than GQA_B200_STATIC_SCRATCH_BYTES */
+#define GQA_B200_ERR_TREE_TOKENS (-15) /* drafted tokens per sequence must be in [1, 64] */
+#define GQA_B200_ERR_ROTATION (-16)   /* rot_dim must be even, in [0, head_dim]; max_position in [0, 2^31) */
+#define GQA_B200_ERR_COMPACT_ROWS (-17) /* at most 1024 rows per sequence in one kv_compact */
 
 /* Workspace header: the first int32 words of the workspace, readable by the
  * host after a stream synchronise when debugging.
@@ -259,6 +262,83 @@ GQA_B200_API int gqa_b200_kv_append(const void* key, const void* value, void* k_
                                     const int32_t* positions, int dtype, int batch, int kv_heads,
                                     int head_dim, int64_t num_blocks, int block_size,
                                     int max_pages, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * The steps around a tree of drafted tokens (speculative decoding) on the same
+ * cache.  None of them has a counterpart in the reference library.
+ * ------------------------------------------------------------------------- */
+
+/* Per-head RMS norm of queries and keys, then the position rotation, in one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight,  (a, b) -> (a cos - b sin, b cos + a sin)
+ * over the first rot_dim elements; the pair is (y[i], y[i + rot_dim/2]), or
+ * (y[2i], y[2i+1]) when `interleaved`.  fp32 inside, one rounding at the end.
+ *   q [batch, tokens, q_heads, head_dim], k and v [.., kv_heads, ..]: any strides
+ *     with unit stride in head_dim; strides = host array of 9 element strides,
+ *     (batch, token, head) of q, of k, of v
+ *   q_weight, k_weight [head_dim] of weight_dtype (= dtype, or GQA_B200_F32); both
+ *     null: no norm
+ *   cos_sin float32 [max_position, rot_dim]: rot_dim/2 cosines, then the sines
+ *   positions int32 [batch, tokens]: row of cos_sin; a token whose position is
+ *     outside [0, max_position) is padding
+ *   q_out [batch, tokens, q_heads, head_dim], contiguous; may be q itself if that
+ *     is contiguous; rows of padding are zeros
+ * k_cache null: dense form, keys go to k_out (as q_out; v and the cache arguments
+ * are ignored).  Otherwise keys and values of token t of sequence b go to position
+ * slots[b, t] of the sequence's pages (layout and block_table as above), nothing is
+ * written for padding, slots outside the table or pages outside the pool.  The
+ * caller owns distinct destinations. */
+GQA_B200_API int gqa_b200_qk_norm_rope(const void* q, const void* k, const void* v,
+                                       const void* q_weight, const void* k_weight,
+                                       const float* cos_sin, const int32_t* positions, void* q_out,
+                                       void* k_out, void* k_cache, void* v_cache,
+                                       const int32_t* block_table, const int32_t* slots, int dtype,
+                                       int weight_dtype, int batch, int tokens, int q_heads,
+                                       int kv_heads, int head_dim, int rot_dim, int64_t max_position,
+                                       const int64_t* strides, float eps, int interleaved,
+                                       int64_t num_blocks, int block_size, int max_pages,
+                                       void* stream);
+
+/* Bytes of scratch gqa_b200_tree_decode needs for this static shape, 256-byte
+ * aligned.  Its contents need not be initialised and nothing carries over between
+ * calls; calls that may overlap on the device need buffers of their own. */
+GQA_B200_API size_t gqa_b200_tree_workspace_bytes(int batch, int tokens, int q_heads, int kv_heads,
+                                                  int head_dim, int block_size, int max_pages);
+
+/* Paged attention of up to 64 drafted tokens per sequence.  q, out are
+ * [batch, tokens, q_heads, head_dim]; context_lens[b] counts the keys in b's pages,
+ * its drafted tokens included: they are the last draft_lens[b] of them (null: all
+ * `tokens`; clamped to [0, tokens]), number j at position
+ * context_lens[b] - draft_lens[b] + j.  Query row i < draft_lens[b] sees every key
+ * before the drafted ones and drafted token j iff bit j of tree_mask[b, i] is set
+ * (int64 [batch, tokens]; null: bits 0 .. i, a chain).  A row that sees nothing, and
+ * rows from draft_lens[b] on, are zeros.  Keys and values that a row does not see
+ * may hold anything, infinities and NaN included.  kernel: GQA_B200_KERNEL_AUTO or
+ * _SIMT. */
+GQA_B200_API int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache,
+                                      const int32_t* block_table, const int32_t* context_lens,
+                                      const int32_t* draft_lens, const int64_t* tree_mask, void* out,
+                                      int dtype, int batch, int tokens, int q_heads, int kv_heads,
+                                      int head_dim, int64_t num_blocks, int block_size,
+                                      int max_pages, float scale, int kernel, void* workspace,
+                                      size_t workspace_bytes, void* stream);
+
+/* Move rows within sequences: the K and V rows at positions src_positions[b, i]
+ * (int32 [batch, n], n <= 1024) go to position dst_positions[b] + i.  Within a
+ * sequence every row is read before any is written.  An entry whose source or
+ * destination is outside the table or on a page outside the pool is skipped (-1:
+ * none).  A row that is written must not belong to another sequence of the call. */
+GQA_B200_API int gqa_b200_kv_compact(void* k_cache, void* v_cache, const int32_t* block_table,
+                                     const int32_t* src_positions, const int32_t* dst_positions,
+                                     int dtype, int batch, int n, int kv_heads, int head_dim,
+                                     int64_t num_blocks, int block_size, int max_pages, void* stream);
+
+/* Copy whole pages of K and V: page src_pages[i] to page dst_pages[i] (int32 [n]).
+ * A pair with an id outside the pool is skipped.  A source may occur often; the
+ * caller owns destinations that are distinct and not also sources. */
+GQA_B200_API int gqa_b200_kv_copy_pages(void* k_cache, void* v_cache, const int32_t* src_pages,
+                                        const int32_t* dst_pages, int dtype, int n, int kv_heads,
+                                        int head_dim, int64_t num_blocks, int block_size,
+                                        void* stream);
 
 #ifdef __cplusplus
 }
