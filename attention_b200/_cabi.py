@@ -35,6 +35,7 @@ SIGNATURES = {
     "gqa_b200_tree_workspace_bytes": (c_size_t, [c_int] * 7),
     "gqa_b200_tree_decode": (c_int, [_P] * 8 + [c_int] * 6 + [c_int64, c_int, c_int, c_float, c_int, _P,
                                                               c_size_t, _P]),
+    "gqa_b200_tree_tc_status": (c_int, [c_int]),
     "gqa_b200_kv_compact": (c_int, [_P] * 5 + [c_int] * 5 + [c_int64, c_int, c_int, _P]),
     "gqa_b200_kv_copy_pages": (c_int, [_P] * 4 + [c_int] * 4 + [c_int64, c_int, _P]),
     # include/mla_decode_b200.h

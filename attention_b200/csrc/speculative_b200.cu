@@ -14,12 +14,14 @@
 
 #include "../../include/gqa_decode_b200.h"
 #include "gqa_tree_simt.cuh"
+#include "gqa_tree_tc.cuh"
 #include "kv_pages.cuh"
 #include "qk_norm_rope.cuh"
 
 namespace gqa_b200 {
 namespace {
 
+constexpr int kMaxDevices = 64;
 constexpr int kSms = 148;                    // the cut of the work is for a B200, whatever runs it
 constexpr int kTreeSimtCtasPerSm = 3;
 constexpr long long kIntMax = 0x7fffffffll;
@@ -116,6 +118,39 @@ TreePlan tree_plan_simt(int batch, int tokens, int q_heads, int kv_heads, long l
                      kTreeSimtCtasPerSm);
 }
 
+
+// Element types, sizes and alignments the tensor-core kernel takes: 16-bit, rows of whole 16-byte
+// chunks, physical row numbers below 2^32.
+bool tree_tc_shape(int dtype, int head_dim, int64_t num_blocks, int block_size) {
+    return dtype != GQA_B200_F32 && head_dim % 8 == 0 && num_blocks * block_size < (1ll << 32);
+}
+int tree_tc_rows(int rows, int head_dim) { return head_dim <= 128 && rows > kTreeBM ? 2 * kTreeBM : kTreeBM; }
+TreePlan tree_plan_tc(int batch, int tokens, int q_heads, int kv_heads, int head_dim, long long cap_tokens) {
+    return tree_plan(batch, tokens, q_heads, kv_heads, cap_tokens,
+                     tree_tc_rows(tokens * (q_heads / kv_heads), head_dim), 1);
+}
+
+// Status word of the tensor-core kernel: 0 ok, 2 = a bounded wait ran out, 3 = the dynamic shared
+// memory base was not 1024-byte aligned.  Read with gqa_b200_tree_tc_status.
+__device__ int g_tree_tc_status;
+int* g_tree_tc_status_ptr[kMaxDevices];
+
+cudaError_t tree_tc_status_address(int** out) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
+    std::lock_guard<std::mutex> lock(g_mutex);
+    if (!g_tree_tc_status_ptr[dev]) {
+        void* ptr = nullptr;
+        e = cudaGetSymbolAddress(&ptr, g_tree_tc_status);
+        if (e != cudaSuccess) return e;
+        g_tree_tc_status_ptr[dev] = static_cast<int*>(ptr);
+    }
+    *out = g_tree_tc_status_ptr[dev];
+    return cudaSuccess;
+}
+
 struct TreeScratch {
     size_t info, ml, acc, total;
 };
@@ -147,13 +182,36 @@ cudaError_t launch_tree_simt_dim(const TreeParams& p, const TreePlan& t, bool ve
     if (p.head_dim <= 128) return launch_tree_simt<T, RB, 128>(p, t, vec, stream);
     return launch_tree_simt<T, RB, 256>(p, t, vec, stream);
 }
+template <typename T, int DP, int NQ>
+cudaError_t launch_tree_tc(const TreeParams& p, const TreePlan& t, cudaStream_t stream) {
+    using G = TreeTcGeom<DP, NQ>;
+    auto kernel = gqa_tree_tc_kernel<T, DP, NQ>;
+    cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), G::kSmemBytes);
+    if (e != cudaSuccess) return e;
+    int* status = nullptr;
+    e = tree_tc_status_address(&status);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(kernel, dim3((unsigned)(t.n_runs * t.units)), G::kThreads, G::kSmemBytes, stream, p, status);
+}
 template <typename T>
-cudaError_t launch_tree(const TreeParams& p, const TreePlan& t, bool vec, cudaStream_t stream) {
-    cudaError_t e;
-    switch (t.row_block) {
-        case 8:  e = launch_tree_simt_dim<T, 8>(p, t, vec, stream); break;
-        case 16: e = launch_tree_simt_dim<T, 16>(p, t, vec, stream); break;
-        default: e = launch_tree_simt_dim<T, 32>(p, t, vec, stream); break;
+cudaError_t launch_tree_tc_dim(const TreeParams& p, const TreePlan& t, cudaStream_t stream) {
+    if (p.head_dim <= 64)
+        return t.row_block == kTreeBM ? launch_tree_tc<T, 64, 1>(p, t, stream) : launch_tree_tc<T, 64, 2>(p, t, stream);
+    if (p.head_dim <= 128)
+        return t.row_block == kTreeBM ? launch_tree_tc<T, 128, 1>(p, t, stream) : launch_tree_tc<T, 128, 2>(p, t, stream);
+    return launch_tree_tc<T, 256, 1>(p, t, stream);
+}
+template <typename T>
+cudaError_t launch_tree(const TreeParams& p, const TreePlan& t, bool tc, bool vec, cudaStream_t stream) {
+    cudaError_t e = cudaErrorInvalidValue;
+    if (tc) {
+        if constexpr (sizeof(T) == 2) e = launch_tree_tc_dim<T>(p, t, stream);
+    } else {
+        switch (t.row_block) {
+            case 8:  e = launch_tree_simt_dim<T, 8>(p, t, vec, stream); break;
+            case 16: e = launch_tree_simt_dim<T, 16>(p, t, vec, stream); break;
+            default: e = launch_tree_simt_dim<T, 32>(p, t, vec, stream); break;
+        }
     }
     if (e != cudaSuccess || t.n_runs == 1) return e;
     const int rows = p.rows * p.kv_heads;
@@ -235,7 +293,9 @@ size_t gqa_b200_tree_workspace_bytes(int batch, int tokens, int q_heads, int kv_
         head_dim <= 0 || head_dim > 256 || block_size <= 0 || max_pages <= 0)
         return 0;
     const long long cap = cap_tokens_of(max_pages, block_size);
-    return tree_scratch(tree_plan_simt(batch, tokens, q_heads, kv_heads, cap), tokens, q_heads, head_dim).total;
+    // either kernel may run: which one depends on types and addresses
+    return std::max(tree_scratch(tree_plan_simt(batch, tokens, q_heads, kv_heads, cap), tokens, q_heads, head_dim).total,
+                    tree_scratch(tree_plan_tc(batch, tokens, q_heads, kv_heads, head_dim, cap), tokens, q_heads, head_dim).total);
 }
 
 int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
@@ -252,12 +312,17 @@ int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache
     if (max_pages <= 0) return GQA_B200_ERR_MAX_PAGES;
     if (!(std::isfinite(scale) && scale > 0.f)) return GQA_B200_ERR_SCALE;
     if (num_blocks > kIntMax || (long long)tokens * q_heads > 65535) return GQA_B200_ERR_INT32_RANGE;
-    if (kernel != GQA_B200_KERNEL_AUTO && kernel != GQA_B200_KERNEL_SIMT) return GQA_B200_ERR_KERNEL;
+    if (kernel != GQA_B200_KERNEL_AUTO && kernel != GQA_B200_KERNEL_SIMT && kernel != GQA_B200_KERNEL_TCGEN05)
+        return GQA_B200_ERR_KERNEL;
     if (batch == 0) return GQA_B200_OK;
     if (!q || !k_cache || !v_cache || !block_table || !context_lens || !out) return GQA_B200_ERR_NULL_POINTER;
 
     const long long cap = cap_tokens_of(max_pages, block_size);
-    const TreePlan plan = tree_plan_simt(batch, tokens, q_heads, kv_heads, cap);
+    const bool tc = kernel != GQA_B200_KERNEL_SIMT && tree_tc_shape(dtype, head_dim, num_blocks, block_size) &&
+                    aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out);
+    if (kernel == GQA_B200_KERNEL_TCGEN05 && !tc) return GQA_B200_ERR_KERNEL;
+    const TreePlan plan = tc ? tree_plan_tc(batch, tokens, q_heads, kv_heads, head_dim, cap)
+                             : tree_plan_simt(batch, tokens, q_heads, kv_heads, cap);
     if (plan.n_runs * plan.units > kIntMax) return GQA_B200_ERR_INT32_RANGE;
     const TreeScratch lay = tree_scratch(plan, tokens, q_heads, head_dim);
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < lay.total)
@@ -282,10 +347,25 @@ int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache
     const bool vec = head_dim * elem_size(dtype) % 16 == 0 && aligned16(q) && aligned16(k_cache) && aligned16(v_cache);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (dtype) {
-        case GQA_B200_F32: return (int)launch_tree<float>(p, plan, vec, s);
-        case GQA_B200_F16: return (int)launch_tree<__half>(p, plan, vec, s);
-        default:           return (int)launch_tree<__nv_bfloat16>(p, plan, vec, s);
+        case GQA_B200_F32: return (int)launch_tree<float>(p, plan, tc, vec, s);
+        case GQA_B200_F16: return (int)launch_tree<__half>(p, plan, tc, vec, s);
+        default:           return (int)launch_tree<__nv_bfloat16>(p, plan, tc, vec, s);
     }
+}
+
+int gqa_b200_tree_tc_status(int reset) {
+    int* status = nullptr;
+    cudaError_t e = tree_tc_status_address(&status);
+    if (e != cudaSuccess) return -(int)e;
+    int host = 0;
+    e = cudaMemcpy(&host, status, sizeof(int), cudaMemcpyDeviceToHost);
+    if (e != cudaSuccess) return -(int)e;
+    if (reset) {
+        const int zero = 0;
+        e = cudaMemcpy(status, &zero, sizeof(int), cudaMemcpyHostToDevice);
+        if (e != cudaSuccess) return -(int)e;
+    }
+    return host;
 }
 
 int gqa_b200_kv_compact(void* k_cache, void* v_cache, const int32_t* block_table, const int32_t* src_positions,

@@ -21,7 +21,7 @@ import torch
 
 from .core import _DTYPE_CODE, _check, _check_cuda_contiguous, _lib, _on_device, _raise_status, _stream_handle
 
-_TREE_KERNEL_CODE = {"auto": 0, "simt": 1}
+_TREE_KERNEL_CODE = {"auto": 0, "simt": 1, "tcgen05": 4}
 _tree_need: dict[tuple, int] = {}
 _Strides = ctypes.c_int64 * 9
 
@@ -184,6 +184,11 @@ def tree_workspace_bytes(batch, tokens, q_heads, kv_heads, head_dim, block_size,
     return int(_lib().gqa_b200_tree_workspace_bytes(batch, tokens, q_heads, kv_heads, head_dim, block_size, max_pages))
 
 
+def tree_tc_status(reset=True) -> int:
+    """Status word of the tcgen05 tree kernel (synchronises): 0 ok, 2 = a bounded wait ran out."""
+    return int(_lib().gqa_b200_tree_tc_status(1 if reset else 0))
+
+
 def gqa_tree_decode(q, k_cache, v_cache, block_table, context_lens, tree_mask=None, *, draft_lens=None, scale=None,
                     out=None, workspace=None, kernel="auto"):
     """Paged GQA attention of up to 64 drafted tokens per sequence.
@@ -195,7 +200,7 @@ def gqa_tree_decode(q, k_cache, v_cache, block_table, context_lens, tree_mask=No
     from ``draft_lens[b]`` on come back as zeros; keys and values that a row does not see may hold
     anything.  ``workspace`` (uint8, at least ``tree_workspace_bytes(...)``, 256-byte aligned, contents
     irrelevant) is taken from the allocator for each call by default, so calls on different streams and
-    captured graphs share nothing.  ``kernel``: ``"auto" | "simt"``.  No autograd support.
+    captured graphs share nothing.  ``kernel``: ``"auto" | "simt" | "tcgen05"``.  No autograd support.
     """
     lib = _lib()
     for t, name in ((q, "q"), (k_cache, "k_cache"), (v_cache, "v_cache"), (block_table, "block_table"),
@@ -234,7 +239,7 @@ def gqa_tree_decode(q, k_cache, v_cache, block_table, context_lens, tree_mask=No
         _check(draft_lens.dtype == torch.int32 and draft_lens.shape == (batch,) and draft_lens.device == dev,
                "draft_lens must be int32 [B] on q's device")
     if kernel not in _TREE_KERNEL_CODE:
-        raise ValueError("kernel must be auto or simt")
+        raise ValueError("kernel must be auto, simt or tcgen05")
     if out is None:
         out = torch.empty_like(q)
     else:

@@ -4,8 +4,8 @@
  * Every entry point takes plain pointers and sizes, never allocates or frees
  * device memory, never throws, and returns an int status: 0 = ok, < 0 = invalid
  * argument (see gqa_b200_strerror), > 0 = a cudaError_t raised by a launch.  No
- * entry point synchronises the device, with two exceptions that say so below:
- * the debug getters gqa_b200_prefill_tc_status and mla_b200_tc_status, which
+ * entry point synchronises the device, with exceptions that say so below:
+ * the debug getters gqa_b200_prefill_tc_status, gqa_b200_tree_tc_status and mla_b200_tc_status, which
  * copy a status word back with a blocking cudaMemcpy.  All device pointers must belong to the
  * device that is current in the calling thread; work is enqueued on `stream`
  * (a cudaStream_t passed as void*; NULL = the legacy default stream).
@@ -312,8 +312,9 @@ GQA_B200_API size_t gqa_b200_tree_workspace_bytes(int batch, int tokens, int q_h
  * before the drafted ones and drafted token j iff bit j of tree_mask[b, i] is set
  * (int64 [batch, tokens]; null: bits 0 .. i, a chain).  A row that sees nothing, and
  * rows from draft_lens[b] on, are zeros.  Keys and values that a row does not see
- * may hold anything, infinities and NaN included.  kernel: GQA_B200_KERNEL_AUTO or
- * _SIMT. */
+ * may hold anything, infinities and NaN included.  kernel: GQA_B200_KERNEL_AUTO,
+ * _SIMT, or _TCGEN05 (fp16/bf16, rows of head_dim elements a multiple of 16 bytes,
+ * 16-byte aligned tensors, num_blocks * block_size < 2^32; what AUTO picks for those). */
 GQA_B200_API int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache,
                                       const int32_t* block_table, const int32_t* context_lens,
                                       const int32_t* draft_lens, const int64_t* tree_mask, void* out,
@@ -321,6 +322,9 @@ GQA_B200_API int gqa_b200_tree_decode(const void* q, const void* k_cache, const 
                                       int head_dim, int64_t num_blocks, int block_size,
                                       int max_pages, float scale, int kernel, void* workspace,
                                       size_t workspace_bytes, void* stream);
+
+/* Debug aid for the tcgen05 tree kernel: as gqa_b200_prefill_tc_status. */
+GQA_B200_API int gqa_b200_tree_tc_status(int reset);
 
 /* Move rows within sequences: the K and V rows at positions src_positions[b, i]
  * (int32 [batch, n], n <= 1024) go to position dst_positions[b] + i.  Within a

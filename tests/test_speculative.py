@@ -30,6 +30,14 @@ DEV = "cuda"
 DTYPES = [torch.float32, torch.float16, torch.bfloat16]
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out(request):
+    """After every GPU test: no bounded wait of the tensor-core kernel gave up."""
+    yield
+    if "gpu" in request.keywords and torch.cuda.is_available():
+        assert attn.speculative.tree_tc_status() == 0
+
+
 def half_step(dtype):
     return torch.finfo(dtype).eps / 2
 
