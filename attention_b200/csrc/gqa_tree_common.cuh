@@ -42,6 +42,7 @@ struct TreeParams {
     int block_size, bs_shift, max_pages;
     long long num_blocks;
     int cap_tokens;
+    int tile_rows;                // tensor-core kernel: rows of a query tile (whole tokens, at most 128)
     float scale_log2;
 };
 
@@ -54,13 +55,14 @@ __device__ __forceinline__ int tree_drafts(const TreeParams& p, int b) {
     const int n = __ldg(p.draft_lens + b);
     return n < 0 ? 0 : (n > p.tokens ? p.tokens : n);
 }
-// Drafted tokens that row token i of n may see (bits of drafted tokens 0 .. n-1).
+// Drafted tokens (bits 0 .. n - 1) that row token i < n may see; `word` is its mask word.
+__device__ __forceinline__ unsigned long long tree_bits_of(const TreeParams& p, unsigned long long word, int i, int n) {
+    const unsigned long long all = n >= 64 ? ~0ull : (1ull << n) - 1ull;
+    return (p.mask ? word : (i >= 63 ? ~0ull : (2ull << i) - 1ull)) & all;
+}
 __device__ __forceinline__ unsigned long long tree_bits(const TreeParams& p, int b, int i, int n) {
     if (i >= n) return 0ull;
-    const unsigned long long all = n >= 64 ? ~0ull : (1ull << n) - 1ull;
-    const unsigned long long m = p.mask ? __ldg(p.mask + (long long)b * p.tokens + i)
-                                        : (i >= 63 ? ~0ull : (2ull << i) - 1ull);
-    return m & all;
+    return tree_bits_of(p, p.mask ? __ldg(p.mask + (long long)b * p.tokens + i) : 0ull, i, n);
 }
 __device__ __forceinline__ int tree_tiles(int len) { return (int)(((long long)len + kTreeTile - 1) / kTreeTile); }
 // Physical row (page * block_size + slot) of a position, the page id clamped into the pool.
@@ -160,64 +162,113 @@ __device__ __forceinline__ long long tree_part_row(const TreeParams& p, int slot
 // Merge: CTA column x stands for the boundary between runs x and x + 1.  If it is the first
 // boundary inside a sequence, the CTA joins that sequence's partials, in run order.
 //   M = max m_r,  out = sum 2^(m_r - M) acc_r / sum 2^(m_r - M) l_r
-// One warp per row; a lane owns columns lane, lane + 32, ...
+// One warp per row.  Lane i looks after piece i of a round of 32 (its maximum, sum and weight), then
+// the warp adds the pieces' rows four at a time, so that a long sequence's many pieces cost a few
+// round trips to memory and not two each (17 pieces x 256 rows: 29 us one after the other).
+// VEC: D is a multiple of 4, a lane owns columns 4 lane .. 4 lane + 3 (and + 128).
 // ---------------------------------------------------------------------------
 constexpr int kTreeMergeWarps = 8;
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(kTreeMergeWarps * 32) gqa_tree_merge_kernel(const TreeParams p) {
     pdl_launch_dependents();
     pdl_wait();
     const int r0 = blockIdx.x;                       // last run before the boundary
     const int4 here = __ldcg(p.info + r0 + 1);
-    if (here.x >= p.batch || here.y == 0) return;    // no tile behind it, or between two sequences
     const int4 prev = __ldcg(p.info + r0);
+    if (here.x >= p.batch || here.y == 0) return;    // no tile behind it, or between two sequences
     if (prev.x == here.x && prev.y != 0) return;     // an earlier boundary is inside this sequence too
     const int b = here.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int tiles = tree_tiles(tree_len(p, b));
-    int r1 = r0 + 1;                                 // last run that holds a piece of b
-    while (r1 + 1 < p.n_ranges) {
-        const int4 nx = __ldcg(p.info + r1 + 1);
-        if (nx.x != b || nx.y >= tiles) break;
-        ++r1;
+    const int slot0 = 2 * r0 + (prev.x == b ? 0 : 1);   // the first piece; every later one begins its run
+    int r1 = r0;                                     // last run that holds a piece of b
+    for (;;) {
+        const int r = r1 + 1 + lane;
+        const bool in = r < p.n_ranges && __ldcg(p.info + r).x == b;
+        const unsigned inside = __ballot_sync(0xffffffffu, in);
+        if (inside == 0xffffffffu) { r1 += 32; continue; }
+        r1 += __ffs(~inside) - 1;
+        break;
     }
     const int n_rows = p.rows * p.kv_heads;
     const int D = p.head_dim;
+    constexpr int NV = VEC ? 2 : 8;                  // groups of columns of a lane
+    constexpr int W = VEC ? 4 : 1;                   // columns of a group
     for (int row = blockIdx.y * kTreeMergeWarps + warp; row < n_rows; row += gridDim.y * kTreeMergeWarps) {
         const int kvh = row / p.rows, rr = row - kvh * p.rows;
-        // a run whose first tile is b's (or that continues b) has its piece in slot 2 r
-        auto slot_of = [&](int r) { return 2 * r + (__ldcg(p.info + r).x == b ? 0 : 1); };
-        float mx = -INFINITY;
-        for (int r = r0; r <= r1; ++r) {
-            if (!__ldcg(p.info + r).z) continue;     // a run without a tile
-            const float2 ml = __ldcg(p.part_ml + tree_part_row(p, slot_of(r), kvh, rr));
-            if (ml.y != 0.f) mx = fmaxf(mx, ml.x);
-        }
-        float acc[8];
+        float acc[NV][W], sum = 0.f, mx = -INFINITY;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j] = 0.f;
-        float sum = 0.f;
-        for (int r = r0; r <= r1; ++r) {
-            if (!__ldcg(p.info + r).z) continue;
-            const long long at = tree_part_row(p, slot_of(r), kvh, rr);
-            const float2 ml = __ldcg(p.part_ml + at);
-            if (ml.y == 0.f) continue;               // nothing visible in this piece
-            const float w = fast_exp2(ml.x - mx);
-            sum += w * ml.y;
-            const float* src = p.part_acc + at * D;
+        for (int j = 0; j < NV; ++j)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int c = lane + 32 * j;
-                if (c < D) acc[j] = fmaf(w, __ldcg(src + c), acc[j]);
+            for (int c = 0; c < W; ++c) acc[j][c] = 0.f;
+        for (int q0 = r0; q0 <= r1; q0 += 32) {
+            const int r = q0 + lane;
+            long long at = 0;
+            float2 ml = make_float2(-INFINITY, 0.f);
+            if (r <= r1 && __ldcg(p.info + r).z) {   // (a run without a tile has no piece)
+                at = tree_part_row(p, r == r0 ? slot0 : 2 * r, kvh, rr);
+                ml = __ldcg(p.part_ml + at);
+            }
+            const bool use = ml.y != 0.f;            // it saw something (NaN counts)
+            float m = use ? ml.x : -INFINITY;
+#pragma unroll
+            for (int x = 16; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+            const unsigned live = __ballot_sync(0xffffffffu, use);
+            if (live == 0) continue;
+            const float mn = fmaxf(mx, m);
+            const float alpha = mx == -INFINITY ? 0.f : fast_exp2(mx - mn);
+            mx = mn;
+            const float w = use ? fast_exp2(ml.x - mn) : 0.f;
+            float s = use ? w * ml.y : 0.f;
+#pragma unroll
+            for (int x = 16; x >= 1; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
+            sum = sum * alpha + s;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int c = 0; c < W; ++c) acc[j][c] *= alpha;
+            for (unsigned todo = live; todo;) {
+                float x[4][NV][W], wt[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int from = todo ? __ffs(todo) - 1 : 0;
+                    const bool has = todo != 0;
+                    todo &= todo - 1;
+                    wt[u] = __shfl_sync(0xffffffffu, w, from);
+                    const float* src = p.part_acc + __shfl_sync(0xffffffffu, at, from) * D;
+#pragma unroll
+                    for (int j = 0; j < NV; ++j) {
+                        const int c = W * (lane + 32 * j);
+                        if (!has || c >= D) {
+#pragma unroll
+                            for (int i = 0; i < W; ++i) x[u][j][i] = 0.f;
+                            continue;
+                        }
+                        if constexpr (VEC) {
+                            const float4 t = __ldcg(reinterpret_cast<const float4*>(src + c));
+                            x[u][j][0] = t.x; x[u][j][1] = t.y; x[u][j][2] = t.z; x[u][j][3] = t.w;
+                        } else {
+                            x[u][j][0] = __ldcg(src + c);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+#pragma unroll
+                    for (int j = 0; j < NV; ++j)
+#pragma unroll
+                        for (int c = 0; c < W; ++c) acc[j][c] = fmaf(wt[u], x[u][j][c], acc[j][c]);
             }
         }
         const int tok = rr / p.group, head = kvh * p.group + rr - tok * p.group;
         T* dst = static_cast<T*>(p.out) + (((long long)b * p.tokens + tok) * p.q_heads + head) * D;
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int c = lane + 32 * j;
-            if (c < D) dst[c] = from_f32<T>(sum == 0.f ? 0.f : acc[j] / sum);
-        }
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const int c = W * (lane + 32 * j) + i;
+                if (c < D) dst[c] = from_f32<T>(sum == 0.f ? 0.f : acc[j][i] * inv);
+            }
     }
 }
 

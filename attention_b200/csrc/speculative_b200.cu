@@ -1,6 +1,7 @@
 // Host side of the speculative-step entry points declared in include/gqa_decode_b200.h: norm and
 // rotation (into pages), tree attention, compaction of an accepted path, page copies.  Argument
 // checks, the cut of the work and the launches.  No allocation, no synchronisation.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -124,10 +125,15 @@ TreePlan tree_plan_simt(int batch, int tokens, int q_heads, int kv_heads, long l
 bool tree_tc_shape(int dtype, int head_dim, int64_t num_blocks, int block_size) {
     return dtype != GQA_B200_F32 && head_dim % 8 == 0 && num_blocks * block_size < (1ll << 32);
 }
-int tree_tc_rows(int rows, int head_dim) { return head_dim <= 128 && rows > kTreeBM ? 2 * kTreeBM : kTreeBM; }
+// Rows of a query tile: as many whole tokens as 128 rows hold (a group of more than 128 heads is cut).
+int tree_tile_rows(int group) { return group <= kTreeBM ? kTreeBM / group * group : kTreeBM; }
+// Two query tiles per CTA share every K and V tile when one does not hold all rows (and two
+// accumulators fit tensor memory).
+int tree_tc_tiles(int rows, int group, int head_dim) { return head_dim <= 128 && rows > tree_tile_rows(group) ? 2 : 1; }
 TreePlan tree_plan_tc(int batch, int tokens, int q_heads, int kv_heads, int head_dim, long long cap_tokens) {
+    const int group = q_heads / kv_heads;
     return tree_plan(batch, tokens, q_heads, kv_heads, cap_tokens,
-                     tree_tc_rows(tokens * (q_heads / kv_heads), head_dim), 1);
+                     tree_tile_rows(group) * tree_tc_tiles(tokens * group, group, head_dim), 1);
 }
 
 // Status word of the tensor-core kernel: 0 ok, 2 = a bounded wait ran out, 3 = the dynamic shared
@@ -182,23 +188,85 @@ cudaError_t launch_tree_simt_dim(const TreeParams& p, const TreePlan& t, bool ve
     if (p.head_dim <= 128) return launch_tree_simt<T, RB, 128>(p, t, vec, stream);
     return launch_tree_simt<T, RB, 256>(p, t, vec, stream);
 }
+// cuTensorMapEncodeTiled, looked up through the runtime so that the library needs no link to the driver.
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return fn;
+}
+
+// A cache as [physical row][kv head][D]; a box is 64 columns of one head x `rows` rows, swizzled as
+// the shared-memory operands are, zeros behind column D.
+bool cache_map(CUtensorMap* map, const void* cache, bool bf16, const TreeParams& p, int rows) {
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return false;
+    const cuuint64_t dims[3] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.kv_heads, (cuuint64_t)p.num_blocks * p.block_size};
+    const cuuint64_t strides[2] = {(cuuint64_t)p.head_dim * 2, (cuuint64_t)p.kv_heads * p.head_dim * 2};
+    const cuuint32_t box[3] = {64, 1, (cuuint32_t)rows}, ones[3] = {1, 1, 1};
+    return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(cache),
+                  dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Queries as [batch * token][kv head][head of the group][D]; a box is 64 columns of a kv head's group x
+// `box_tokens` tokens.  (Tokens behind a sequence's last belong to rows that nobody reads.)
+bool query_map(CUtensorMap* map, bool bf16, const TreeParams& p, int box_tokens) {
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return false;
+    const cuuint64_t row = (cuuint64_t)p.head_dim * 2;
+    const cuuint64_t dims[4] = {(cuuint64_t)p.head_dim, (cuuint64_t)p.group, (cuuint64_t)p.kv_heads, (cuuint64_t)p.batch * p.tokens};
+    const cuuint64_t strides[3] = {row, row * p.group, row * p.q_heads};
+    const cuuint32_t box[4] = {64, (cuuint32_t)p.group, 1, (cuuint32_t)box_tokens}, ones[4] = {1, 1, 1, 1};
+    return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(p.q), dims,
+                  strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename T, int DP, int NQ>
 cudaError_t launch_tree_tc(const TreeParams& p, const TreePlan& t, cudaStream_t stream) {
-    using G = TreeTcGeom<DP, NQ>;
-    auto kernel = gqa_tree_tc_kernel<T, DP, NQ>;
-    cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), G::kSmemBytes);
-    if (e != cudaSuccess) return e;
     int* status = nullptr;
-    e = tree_tc_status_address(&status);
+    cudaError_t e = tree_tc_status_address(&status);
     if (e != cudaSuccess) return e;
-    return launch_pdl(kernel, dim3((unsigned)(t.n_runs * t.units)), G::kThreads, G::kSmemBytes, stream, p, status);
+    // Pages by TMA: a box of whole 8-row groups, a tile of whole boxes or a page of whole tiles, row
+    // numbers that are int32 coordinates, and tiles of whole tokens.
+    constexpr int BN = TreeTcGeom<DP, NQ, true>::kBN;
+    CUtensorMap map_q{}, map_k{}, map_v{};
+    bool tma = p.block_size % 8 == 0 && (BN % p.block_size == 0 || p.block_size % BN == 0) &&
+               p.num_blocks * p.block_size <= kIntMax && p.group <= kTreeBM && (long long)p.batch * p.tokens <= kIntMax;
+    if (tma) {
+        const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+        const int rows = std::min(p.block_size, BN);
+        tma = cache_map(&map_k, p.k, bf16, p, rows) && cache_map(&map_v, p.v, bf16, p, rows) &&
+              query_map(&map_q, bf16, p, std::min(p.tokens, p.tile_rows / p.group));
+    }
+    const dim3 grid((unsigned)(t.n_runs * t.units));
+    if (tma) {
+        using G = TreeTcGeom<DP, NQ, true>;
+        auto kernel = gqa_tree_tc_kernel<T, DP, NQ, true>;
+        e = allow_smem(reinterpret_cast<const void*>(kernel), G::kSmemBytes);
+        if (e != cudaSuccess) return e;
+        return launch_pdl(kernel, grid, G::kThreads, G::kSmemBytes, stream, p, map_q, map_k, map_v, status);
+    }
+    using G = TreeTcGeom<DP, NQ, false>;
+    auto kernel = gqa_tree_tc_kernel<T, DP, NQ, false>;
+    e = allow_smem(reinterpret_cast<const void*>(kernel), G::kSmemBytes);
+    if (e != cudaSuccess) return e;
+    return launch_pdl(kernel, grid, G::kThreads, G::kSmemBytes, stream, p, map_q, map_k, map_v, status);
 }
 template <typename T>
 cudaError_t launch_tree_tc_dim(const TreeParams& p, const TreePlan& t, cudaStream_t stream) {
-    if (p.head_dim <= 64)
-        return t.row_block == kTreeBM ? launch_tree_tc<T, 64, 1>(p, t, stream) : launch_tree_tc<T, 64, 2>(p, t, stream);
-    if (p.head_dim <= 128)
-        return t.row_block == kTreeBM ? launch_tree_tc<T, 128, 1>(p, t, stream) : launch_tree_tc<T, 128, 2>(p, t, stream);
+    const bool two = t.row_block > p.tile_rows;
+    if (p.head_dim <= 64) return two ? launch_tree_tc<T, 64, 2>(p, t, stream) : launch_tree_tc<T, 64, 1>(p, t, stream);
+    if (p.head_dim <= 128) return two ? launch_tree_tc<T, 128, 2>(p, t, stream) : launch_tree_tc<T, 128, 1>(p, t, stream);
     return launch_tree_tc<T, 256, 1>(p, t, stream);
 }
 template <typename T>
@@ -216,8 +284,8 @@ cudaError_t launch_tree(const TreeParams& p, const TreePlan& t, bool tc, bool ve
     if (e != cudaSuccess || t.n_runs == 1) return e;
     const int rows = p.rows * p.kv_heads;
     const int by = std::min((rows + kTreeMergeWarps - 1) / kTreeMergeWarps, 65535);
-    return launch_pdl(gqa_tree_merge_kernel<T>, dim3((unsigned)(t.n_runs - 1), (unsigned)by), kTreeMergeWarps * 32, 0,
-                      stream, p);
+    auto merge = p.head_dim % 4 == 0 ? gqa_tree_merge_kernel<T, true> : gqa_tree_merge_kernel<T, false>;
+    return launch_pdl(merge, dim3((unsigned)(t.n_runs - 1), (unsigned)by), kTreeMergeWarps * 32, 0, stream, p);
 }
 
 // ---------------------------------------------------------------------------
@@ -337,7 +405,7 @@ int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache
     p.part_acc = reinterpret_cast<float*>(ws + lay.acc);
     p.n_ranges = plan.n_runs;
     p.batch = batch; p.tokens = tokens; p.q_heads = q_heads; p.kv_heads = kv_heads; p.group = q_heads / kv_heads;
-    p.head_dim = head_dim; p.rows = tokens * p.group; p.row_blocks = plan.row_blocks;
+    p.head_dim = head_dim; p.rows = tokens * p.group; p.row_blocks = plan.row_blocks; p.tile_rows = tree_tile_rows(p.group);
     p.block_size = block_size; p.max_pages = max_pages; p.num_blocks = num_blocks;
     p.bs_shift = -1;
     for (int s = 0; s < 31; ++s)

@@ -223,7 +223,7 @@ def check_tree(got, case, scale=None):
 @pytest.mark.parametrize("kernel", ["auto", "simt"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("t,hq,hkv", [(1, 8, 8), (1, 8, 2), (3, 5, 5), (8, 8, 2), (16, 14, 2), (33, 8, 1), (64, 4, 2),
-                                      (9, 64, 4)])
+                                      (9, 64, 4), (3, 130, 1), (2, 128, 1), (20, 15, 1), (43, 6, 2)])
 def test_tree_heads_and_tokens(dtype, t, hq, hkv, kernel):
     case = tree_case([t, 70 + t, 300, 129], t, hq, hkv, 128, 16, dtype, seed=t)
     dc = on_gpu(*case)
@@ -233,7 +233,7 @@ def test_tree_heads_and_tokens(dtype, t, hq, hkv, kernel):
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("d,bs", [(128, 1), (64, 5), (96, 24), (80, 16), (40, 16), (8, 8), (256, 32), (200, 64), (37, 7),
-                                  (1, 16)])
+                                  (1, 16), (128, 8), (64, 128), (128, 256), (256, 8), (72, 16), (136, 384), (24, 32)])
 def test_tree_head_dims_and_pages(dtype, d, bs):
     case = tree_case([5, 64, 257], 5, 6, 2, d, bs, dtype, seed=d)
     dc = on_gpu(*case)
