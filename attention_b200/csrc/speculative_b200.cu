@@ -125,15 +125,22 @@ TreePlan tree_plan_simt(int batch, int tokens, int q_heads, int kv_heads, long l
 bool tree_tc_shape(int dtype, int head_dim, int64_t num_blocks, int block_size) {
     return dtype != GQA_B200_F32 && head_dim % 8 == 0 && num_blocks * block_size < (1ll << 32);
 }
+int tree_tc_keys(int head_dim) { return head_dim <= 128 ? 128 : 64; }      // of an inner tile
+// Pages by TMA: a box of whole 8-row groups, a tile of whole boxes or a page of whole tiles, row numbers
+// that are int32 coordinates, and query tiles of whole tokens.
+bool tree_tma_shape(int group, int head_dim, int64_t num_blocks, int block_size, long long query_tokens) {
+    const int bn = tree_tc_keys(head_dim);
+    return block_size % 8 == 0 && (bn % block_size == 0 || block_size % bn == 0) && num_blocks * block_size <= kIntMax &&
+           group <= kTreeBM && query_tokens <= kIntMax;
+}
 // Rows of a query tile: as many whole tokens as 128 rows hold (a group of more than 128 heads is cut).
 int tree_tile_rows(int group) { return group <= kTreeBM ? kTreeBM / group * group : kTreeBM; }
-// Two query tiles per CTA share every K and V tile when one does not hold all rows (and two
-// accumulators fit tensor memory).
-int tree_tc_tiles(int rows, int group, int head_dim) { return head_dim <= 128 && rows > tree_tile_rows(group) ? 2 : 1; }
-TreePlan tree_plan_tc(int batch, int tokens, int q_heads, int kv_heads, int head_dim, long long cap_tokens) {
-    const int group = q_heads / kv_heads;
-    return tree_plan(batch, tokens, q_heads, kv_heads, cap_tokens,
-                     tree_tile_rows(group) * tree_tc_tiles(tokens * group, group, head_dim), 1);
+// Two query tiles per CTA share every K and V tile when one does not hold all rows (if the keys come by
+// TMA, and two accumulators fit tensor memory).
+TreePlan tree_plan_tc(int batch, int tokens, int q_heads, int kv_heads, int head_dim, long long cap_tokens, bool tma) {
+    const int group = q_heads / kv_heads, tile = tree_tile_rows(group);
+    const int tiles = tma && head_dim <= 128 && tokens * group > tile ? 2 : 1;
+    return tree_plan(batch, tokens, q_heads, kv_heads, cap_tokens, tile * tiles, 1);
 }
 
 // Status word of the tensor-core kernel: 0 ok, 2 = a bounded wait ran out, 3 = the dynamic shared
@@ -231,49 +238,47 @@ bool query_map(CUtensorMap* map, bool bf16, const TreeParams& p, int box_tokens)
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int DP, int NQ>
-cudaError_t launch_tree_tc(const TreeParams& p, const TreePlan& t, cudaStream_t stream) {
+struct TreeMaps {
+    CUtensorMap q, k, v;
+};
+bool tree_maps(TreeMaps* m, bool bf16, const TreeParams& p) {
+    const int rows = std::min(p.block_size, tree_tc_keys(p.head_dim));
+    return cache_map(&m->k, p.k, bf16, p, rows) && cache_map(&m->v, p.v, bf16, p, rows) &&
+           query_map(&m->q, bf16, p, std::min(p.tokens, p.tile_rows / p.group));
+}
+
+template <typename T, int DP, int MODE, bool TMA>
+cudaError_t launch_tree_tc(const TreeParams& p, const TreePlan& t, const TreeMaps& maps, cudaStream_t stream) {
     int* status = nullptr;
     cudaError_t e = tree_tc_status_address(&status);
     if (e != cudaSuccess) return e;
-    // Pages by TMA: a box of whole 8-row groups, a tile of whole boxes or a page of whole tiles, row
-    // numbers that are int32 coordinates, and tiles of whole tokens.
-    constexpr int BN = TreeTcGeom<DP, NQ, true>::kBN;
-    CUtensorMap map_q{}, map_k{}, map_v{};
-    bool tma = p.block_size % 8 == 0 && (BN % p.block_size == 0 || p.block_size % BN == 0) &&
-               p.num_blocks * p.block_size <= kIntMax && p.group <= kTreeBM && (long long)p.batch * p.tokens <= kIntMax;
-    if (tma) {
-        const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
-        const int rows = std::min(p.block_size, BN);
-        tma = cache_map(&map_k, p.k, bf16, p, rows) && cache_map(&map_v, p.v, bf16, p, rows) &&
-              query_map(&map_q, bf16, p, std::min(p.tokens, p.tile_rows / p.group));
-    }
-    const dim3 grid((unsigned)(t.n_runs * t.units));
-    if (tma) {
-        using G = TreeTcGeom<DP, NQ, true>;
-        auto kernel = gqa_tree_tc_kernel<T, DP, NQ, true>;
-        e = allow_smem(reinterpret_cast<const void*>(kernel), G::kSmemBytes);
-        if (e != cudaSuccess) return e;
-        return launch_pdl(kernel, grid, G::kThreads, G::kSmemBytes, stream, p, map_q, map_k, map_v, status);
-    }
-    using G = TreeTcGeom<DP, NQ, false>;
-    auto kernel = gqa_tree_tc_kernel<T, DP, NQ, false>;
+    using G = TreeTcGeom<DP, MODE>;
+    static_assert(G::kBN == (DP <= 128 ? 128 : 64), "tree_tc_keys");
+    auto kernel = gqa_tree_tc_kernel<T, DP, MODE, TMA>;
     e = allow_smem(reinterpret_cast<const void*>(kernel), G::kSmemBytes);
     if (e != cudaSuccess) return e;
-    return launch_pdl(kernel, grid, G::kThreads, G::kSmemBytes, stream, p, map_q, map_k, map_v, status);
+    return launch_pdl(kernel, dim3((unsigned)(t.n_runs * t.units)), kTreeTcWarps<MODE, TMA> * 32, G::kSmemBytes, stream, p,
+                      maps.q, maps.k, maps.v, status);
 }
 template <typename T>
-cudaError_t launch_tree_tc_dim(const TreeParams& p, const TreePlan& t, cudaStream_t stream) {
+cudaError_t launch_tree_tc_dim(const TreeParams& p, const TreePlan& t, const TreeMaps* maps, cudaStream_t stream) {
+    const int d = p.head_dim;
+    if (!maps) {
+        const TreeMaps none{};
+        if (d <= 64) return launch_tree_tc<T, 64, 0, false>(p, t, none, stream);
+        if (d <= 128) return launch_tree_tc<T, 128, 0, false>(p, t, none, stream);
+        return launch_tree_tc<T, 256, 0, false>(p, t, none, stream);
+    }
     const bool two = t.row_block > p.tile_rows;
-    if (p.head_dim <= 64) return two ? launch_tree_tc<T, 64, 2>(p, t, stream) : launch_tree_tc<T, 64, 1>(p, t, stream);
-    if (p.head_dim <= 128) return two ? launch_tree_tc<T, 128, 2>(p, t, stream) : launch_tree_tc<T, 128, 1>(p, t, stream);
-    return launch_tree_tc<T, 256, 1>(p, t, stream);
+    if (d <= 64) return two ? launch_tree_tc<T, 64, 2, true>(p, t, *maps, stream) : launch_tree_tc<T, 64, 1, true>(p, t, *maps, stream);
+    if (d <= 128) return two ? launch_tree_tc<T, 128, 2, true>(p, t, *maps, stream) : launch_tree_tc<T, 128, 1, true>(p, t, *maps, stream);
+    return launch_tree_tc<T, 256, 0, true>(p, t, *maps, stream);
 }
 template <typename T>
-cudaError_t launch_tree(const TreeParams& p, const TreePlan& t, bool tc, bool vec, cudaStream_t stream) {
+cudaError_t launch_tree(const TreeParams& p, const TreePlan& t, bool tc, const TreeMaps* maps, bool vec, cudaStream_t stream) {
     cudaError_t e = cudaErrorInvalidValue;
     if (tc) {
-        if constexpr (sizeof(T) == 2) e = launch_tree_tc_dim<T>(p, t, stream);
+        if constexpr (sizeof(T) == 2) e = launch_tree_tc_dim<T>(p, t, maps, stream);
     } else {
         switch (t.row_block) {
             case 8:  e = launch_tree_simt_dim<T, 8>(p, t, vec, stream); break;
@@ -361,9 +366,13 @@ size_t gqa_b200_tree_workspace_bytes(int batch, int tokens, int q_heads, int kv_
         head_dim <= 0 || head_dim > 256 || block_size <= 0 || max_pages <= 0)
         return 0;
     const long long cap = cap_tokens_of(max_pages, block_size);
-    // either kernel may run: which one depends on types and addresses
-    return std::max(tree_scratch(tree_plan_simt(batch, tokens, q_heads, kv_heads, cap), tokens, q_heads, head_dim).total,
-                    tree_scratch(tree_plan_tc(batch, tokens, q_heads, kv_heads, head_dim, cap), tokens, q_heads, head_dim).total);
+    // any of the kernels may run: which one depends on types, addresses and the size of the pool
+    const TreePlan plans[3] = {tree_plan_simt(batch, tokens, q_heads, kv_heads, cap),
+                               tree_plan_tc(batch, tokens, q_heads, kv_heads, head_dim, cap, false),
+                               tree_plan_tc(batch, tokens, q_heads, kv_heads, head_dim, cap, true)};
+    size_t need = 0;
+    for (const TreePlan& t : plans) need = std::max(need, tree_scratch(t, tokens, q_heads, head_dim).total);
+    return need;
 }
 
 int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
@@ -389,23 +398,12 @@ int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache
     const bool tc = kernel != GQA_B200_KERNEL_SIMT && tree_tc_shape(dtype, head_dim, num_blocks, block_size) &&
                     aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out);
     if (kernel == GQA_B200_KERNEL_TCGEN05 && !tc) return GQA_B200_ERR_KERNEL;
-    const TreePlan plan = tc ? tree_plan_tc(batch, tokens, q_heads, kv_heads, head_dim, cap)
-                             : tree_plan_simt(batch, tokens, q_heads, kv_heads, cap);
-    if (plan.n_runs * plan.units > kIntMax) return GQA_B200_ERR_INT32_RANGE;
-    const TreeScratch lay = tree_scratch(plan, tokens, q_heads, head_dim);
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < lay.total)
-        return GQA_B200_ERR_WORKSPACE;
-    char* ws = static_cast<char*>(workspace);
     TreeParams p{};
     p.q = q; p.k = k_cache; p.v = v_cache; p.out = out;
     p.table = block_table; p.lens = context_lens; p.draft_lens = draft_lens;
     p.mask = reinterpret_cast<const unsigned long long*>(tree_mask);
-    p.info = reinterpret_cast<int4*>(ws + lay.info);
-    p.part_ml = reinterpret_cast<float2*>(ws + lay.ml);
-    p.part_acc = reinterpret_cast<float*>(ws + lay.acc);
-    p.n_ranges = plan.n_runs;
     p.batch = batch; p.tokens = tokens; p.q_heads = q_heads; p.kv_heads = kv_heads; p.group = q_heads / kv_heads;
-    p.head_dim = head_dim; p.rows = tokens * p.group; p.row_blocks = plan.row_blocks; p.tile_rows = tree_tile_rows(p.group);
+    p.head_dim = head_dim; p.rows = tokens * p.group; p.tile_rows = tree_tile_rows(p.group);
     p.block_size = block_size; p.max_pages = max_pages; p.num_blocks = num_blocks;
     p.bs_shift = -1;
     for (int s = 0; s < 31; ++s)
@@ -413,11 +411,26 @@ int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache
     p.cap_tokens = (int)cap;
     p.scale_log2 = scale * kLog2e;
     const bool vec = head_dim * elem_size(dtype) % 16 == 0 && aligned16(q) && aligned16(k_cache) && aligned16(v_cache);
+    TreeMaps maps{};
+    const bool tma = tc && tree_tma_shape(p.group, head_dim, num_blocks, block_size, (long long)batch * tokens) &&
+                     tree_maps(&maps, dtype == GQA_B200_BF16, p);
+    const TreePlan plan = tc ? tree_plan_tc(batch, tokens, q_heads, kv_heads, head_dim, cap, tma)
+                             : tree_plan_simt(batch, tokens, q_heads, kv_heads, cap);
+    if (plan.n_runs * plan.units > kIntMax) return GQA_B200_ERR_INT32_RANGE;
+    const TreeScratch lay = tree_scratch(plan, tokens, q_heads, head_dim);
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < lay.total)
+        return GQA_B200_ERR_WORKSPACE;
+    char* ws = static_cast<char*>(workspace);
+    p.info = reinterpret_cast<int4*>(ws + lay.info);
+    p.part_ml = reinterpret_cast<float2*>(ws + lay.ml);
+    p.part_acc = reinterpret_cast<float*>(ws + lay.acc);
+    p.n_ranges = plan.n_runs;
+    p.row_blocks = plan.row_blocks;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (dtype) {
-        case GQA_B200_F32: return (int)launch_tree<float>(p, plan, tc, vec, s);
-        case GQA_B200_F16: return (int)launch_tree<__half>(p, plan, tc, vec, s);
-        default:           return (int)launch_tree<__nv_bfloat16>(p, plan, tc, vec, s);
+        case GQA_B200_F32: return (int)launch_tree<float>(p, plan, tc, tma ? &maps : nullptr, vec, s);
+        case GQA_B200_F16: return (int)launch_tree<__half>(p, plan, tc, tma ? &maps : nullptr, vec, s);
+        default:           return (int)launch_tree<__nv_bfloat16>(p, plan, tc, tma ? &maps : nullptr, vec, s);
     }
 }
 
