@@ -201,15 +201,13 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
     // barrier's number, the warp.
     bool alive = true;
     auto wait_bar = [&](uint32_t bar, uint32_t parity) {
-        // (the vote also brings the warp together again: the tensor-memory instructions behind need that)
-        if (__all_sync(0xffffffffu, !alive || tc::mbar_test(bar, parity))) return;
+        if (tc::mbar_test(bar, parity)) return;
         const bool dead = *reinterpret_cast<volatile int*>(&s_dead) != 0;
-        if (!tc::mbar_wait(bar, parity, dead ? 1000ull : 1000000000ull)) {
+        if (alive && !tc::mbar_wait(bar, parity, dead ? 1000ull : 1000000000ull)) {
             *reinterpret_cast<volatile int*>(&s_dead) = 1;
             alive = false;
             if (!dead) atomicCAS(status, 0, 2 | (int)((bar - q_full) >> 3) << 8 | warp << 16);
         }
-        alive = __all_sync(0xffffffffu, alive);
     };
 
     // 16-byte chunk of a row that this lane copies, and the rows a pass of the warp covers
@@ -244,7 +242,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
     int C0[2] = {0, 0};                              // the chains' running numbers of their tiles
     uint32_t k_par = 0, v_par = 0;                   // bit s: parity of the chain's next use of stage s
     int piece = 0;
-    long long left = run.count;
+    int left = (int)run.count;                       // (fits: the launcher checks it)
     int first = run.first;
     // what a piece needs of its sequence is asked for a piece ahead
     const int row = row0 + (MODE == 2 ? X * p.tile_rows : 0) + quad * 32 + lane;   // softmax threads
@@ -266,7 +264,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
         ask_sequence(b + 1);
         const int tiles = tree_tiles(len);
         if (tiles == 0) continue;
-        const int take = (int)(left < tiles - first ? left : tiles - first);
+        const int take = min(left, tiles - first);
         left -= take;
         const bool whole = take == tiles;
         const int t0 = first * kTreeTile, t1 = min(len, (first + take) * kTreeTile);
@@ -466,7 +464,6 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
             if (tid == 0) s_bad[(piece + 8) % kTreeBadRing] = 0ull;
             float m_run = -INFINITY, l_run = 0.f;
             const int nx = tiles_of(X), c0 = X ? C0[1] : C0[0];
-
             for (int i = 0; i < nx; ++i) {
                 const int C = c0 + i;                            // running number: parity of the hand-offs
                 const int stage = (J0 + tile_of(X, i)) % NSV;
@@ -475,6 +472,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     wait_bar(bar_s + (X * 2 + h) * 8, C & 1);
+                    __syncwarp();                                // the tensor-memory instructions want the whole warp
                     tc::tc_fence_after();
                     const int t_base = t0 + tile_of(X, i) * BN + h * HN;
                     float sc[HN];
@@ -520,12 +518,10 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                         l_run *= alpha;
                     }
                     const float nref = m_run == -INFINITY ? 0.f : -m_run;
-                    // exponents, then the exponentials in place (volatile, so that pairs stay pairs), then
-                    // sums and conversions: the packed forms need no register moves this way
 #pragma unroll
                     for (int c = 0; c < HN; c += 2) tc::fma2(sc[c], sc[c + 1], sc[c], sc[c + 1], p.scale_log2, nref);
 #pragma unroll
-                    for (int c = 0; c < HN; ++c) asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(sc[c]));
+                    for (int c = 0; c < HN; ++c) sc[c] = fast_exp2(sc[c]);
                     uint32_t pw[HN / 2];
                     float ps0 = 0.f, ps1 = 0.f;
 #pragma unroll
@@ -537,6 +533,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                     // O_X may be rescaled once P.V of the half before is done
                     if ((i > 0 || h > 0) && __any_sync(0xffffffffu, need)) {
                         wait_bar(bar_o + (X * 2 + (h ^ 1)) * 8, (h ? C : C - 1) & 1);
+                        __syncwarp();
                         tc::tc_fence_after();
 #pragma unroll
                         for (int c0 = 0; c0 < DP; c0 += 32) {

@@ -416,7 +416,8 @@ int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache
                      tree_maps(&maps, dtype == GQA_B200_BF16, p);
     const TreePlan plan = tc ? tree_plan_tc(batch, tokens, q_heads, kv_heads, head_dim, cap, tma)
                              : tree_plan_simt(batch, tokens, q_heads, kv_heads, cap);
-    if (plan.n_runs * plan.units > kIntMax) return GQA_B200_ERR_INT32_RANGE;
+    const long long cap_tiles = (long long)batch * ((cap + kTreeTile - 1) / kTreeTile);
+    if (plan.n_runs * plan.units > kIntMax || cap_tiles / plan.n_runs >= kIntMax / 2) return GQA_B200_ERR_INT32_RANGE;
     const TreeScratch lay = tree_scratch(plan, tokens, q_heads, head_dim);
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < lay.total)
         return GQA_B200_ERR_WORKSPACE;
