@@ -296,9 +296,43 @@ cudaError_t launch_tree(const TreeParams& p, const TreePlan& t, bool tc, const T
 // ---------------------------------------------------------------------------
 // norm and rotation
 // ---------------------------------------------------------------------------
+template <typename T, int L, int HB>
+cudaError_t launch_rope_vec(const RopeParams& p, int heads, cudaStream_t stream) {
+    const int blocks = (heads + HB - 1) / HB;
+    const long long groups = kRopeThreads / L;
+    const long long grid = (p.n_tokens * blocks + groups - 1) / groups;
+    if (grid > kIntMax) return cudaErrorInvalidValue;
+    auto kernel = p.interleaved ? qk_norm_rope_vec_kernel<T, L, HB, true> : qk_norm_rope_vec_kernel<T, L, HB, false>;
+    kernel<<<(unsigned)grid, kRopeThreads, 0, stream>>>(p, blocks);
+    return cudaGetLastError();
+}
+template <typename T, int L>
+cudaError_t launch_rope_heads(const RopeParams& p, int heads, cudaStream_t stream) {
+    // four heads per group once that still gives every SM its fill of threads
+    return p.n_tokens * heads * L >= 4ll * kSms * 2048 ? launch_rope_vec<T, L, 4>(p, heads, stream)
+                                                       : launch_rope_vec<T, L, 1>(p, heads, stream);
+}
+
+// The vector kernel takes rows of whole eight-element chunks, 16-byte aligned throughout, with the
+// rotation's halves (or pairs) in whole chunks.
+bool rope_vec_ok(const RopeParams& p, int size) {
+    const long long strides[9] = {p.q_sb, p.q_st, p.q_sh, p.k_sb, p.k_st, p.k_sh, p.v_sb, p.v_st, p.v_sh};
+    for (int i = 0; i < (p.append ? 9 : 6); ++i)
+        if (strides[i] * size % 16 != 0) return false;
+    const void* ptrs[10] = {p.q, p.k, p.v, p.q_weight, p.k_weight, p.cos_sin, p.q_out, p.k_out, p.k_cache, p.v_cache};
+    for (const void* x : ptrs)
+        if (!aligned16(x)) return false;
+    return p.head_dim % 8 == 0 && p.rot_dim % (p.interleaved ? 8 : 16) == 0;
+}
+
 template <typename T>
 cudaError_t launch_rope(const RopeParams& p, cudaStream_t stream) {
     const int heads = p.q_heads + p.kv_heads * (p.append ? 2 : 1);
+    if (rope_vec_ok(p, (int)sizeof(T))) {
+        if (p.head_dim <= 64) return launch_rope_heads<T, 8>(p, heads, stream);
+        if (p.head_dim <= 128) return launch_rope_heads<T, 16>(p, heads, stream);
+        return launch_rope_heads<T, 32>(p, heads, stream);
+    }
     const long long rows = p.n_tokens * heads;
     const long long grid = (rows + kRopeWarps - 1) / kRopeWarps;
     if (grid > kIntMax) return cudaErrorInvalidValue;
