@@ -11,6 +11,8 @@
 // id outside the pool is skipped, as in kv_append.
 #pragma once
 
+#include <type_traits>
+
 #include "gqa_common.cuh"
 
 namespace gqa_b200 {
@@ -145,146 +147,182 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_any_kernel(const
 }
 
 // ---------------------------------------------------------------------------
-// Rows of whole 16-byte chunks, aligned: a group of L lanes per head row, eight consecutive elements
-// per lane, HB heads of a token one after the other.  All loads of the HB rows are issued before the
-// first is used.  The token's cosines and sines are loaded once for the HB heads (for eight 16-bit
-// elements they are as many as 64 bytes against 16: one head per group is bound by the first-level
-// cache, see the launcher).  The partner of an element is in the same lane (interleaved) or rot_dim/2
-// elements away, rot_dim/16 lanes, so a shuffle fetches it after the scaling.
-// Memory bound: 2 bytes read and 2 written per element of 16 bits.
+// Aligned rows of whole eight-element chunks: a group of L lanes per head row, two chunks of four
+// elements per lane, HB heads of a token one after the other.  The chunks are chosen so that both
+// elements of a pair are in the lane: 4 l and rot_dim/2 + 4 l (halves), or 8 l and 8 l + 4 (interleaved,
+// and behind rot_dim); a lane needs four cosines and four sines, and nothing crosses lanes but the sum.
+// (With eight consecutive elements per lane the partner came by shuffle and a lane read 64 bytes of
+// angles: 190 us for 16384 tokens of 72 heads of 128 16-bit elements.)  All loads of the HB rows are
+// issued before the first is used, the angles are loaded once for all of them.
+// Memory bound: 2 bytes read and 2 written per element of 16 bits (116 us for those tokens, 0.80 of the
+// measured copy bandwidth; float32 1.0), and not far from the issue rate, hence the packed fp32 forms.
 // ---------------------------------------------------------------------------
 constexpr int kRopeThreads = 256;
 
-template <typename T> struct RopeVec {                 // eight elements of a lane
-    uint4 raw[sizeof(T) / 2];
-    __device__ __forceinline__ void load(const T* p) {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = reinterpret_cast<const uint4*>(p)[i];
+template <typename T> struct RopeVec {                 // two chunks of four elements
+    using Chunk = typename std::conditional<sizeof(T) == 2, uint2, uint4>::type;
+    Chunk c[2];
+    __device__ __forceinline__ void load(const T* p, int e0, int e1) {
+        c[0] = *reinterpret_cast<const Chunk*>(p + e0);
+        c[1] = *reinterpret_cast<const Chunk*>(p + e1);
     }
-    __device__ __forceinline__ void store(T* p) const {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(p)[i] = raw[i];
+    __device__ __forceinline__ void store(T* p, int e0, int e1) const {
+        *reinterpret_cast<Chunk*>(p + e0) = c[0];
+        *reinterpret_cast<Chunk*>(p + e1) = c[1];
     }
     __device__ __forceinline__ void get(float (&x)[8]) const {
-        const T* e = reinterpret_cast<const T*>(raw);
+        const T* e = reinterpret_cast<const T*>(c);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = to_f32<T>(e[i]);
     }
     __device__ __forceinline__ void set(const float (&x)[8]) {
-        T* e = reinterpret_cast<T*>(raw);
+        T* e = reinterpret_cast<T*>(c);
 #pragma unroll
         for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(x[i]);
     }
 };
 
+// packed fp32 pairs: half the instructions of the scalar forms
+__device__ __forceinline__ void rope_mul2(float* d, const float* a, const float* b) {
+    asm("{\n\t.reg .b64 ra, rb;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\t"
+        "mul.rn.f32x2 ra, ra, rb;\n\tmov.b64 {%0, %1}, ra;\n\t}"
+        : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]));
+}
+__device__ __forceinline__ void rope_fma2(float* d, const float* a, const float* b, const float* c) {
+    asm("{\n\t.reg .b64 ra, rb, rc;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+        "fma.rn.f32x2 ra, ra, rb, rc;\n\tmov.b64 {%0, %1}, ra;\n\t}"
+        : "=f"(d[0]), "=f"(d[1]) : "f"(a[0]), "f"(a[1]), "f"(b[0]), "f"(b[1]), "f"(c[0]), "f"(c[1]));
+}
+
+// A token has blocks of HB query heads, then of key heads, then (append form) of value heads.
+struct RopeBlocks {
+    unsigned q, k, all;
+};
+
 template <typename T, int L, int HB, bool INTERLEAVED>
-__global__ void __launch_bounds__(kRopeThreads) qk_norm_rope_vec_kernel(const RopeParams p, const int blocks_per_token) {
-    constexpr int GROUPS = kRopeThreads / L;
+__global__ void __launch_bounds__(kRopeThreads, 4)
+qk_norm_rope_vec_kernel(const RopeParams p, const RopeBlocks blocks, const unsigned units) {
+    constexpr unsigned GROUPS = kRopeThreads / L;
     const int lane = threadIdx.x % L;
-    const long long unit = (long long)blockIdx.x * GROUPS + threadIdx.x / L;
-    const long long units = p.n_tokens * blocks_per_token;
+    const unsigned unit = blockIdx.x * GROUPS + threadIdx.x / L;
     const bool work = unit < units;                    // (no early return: the shuffles name whole warps)
-    const long long token = work ? unit / blocks_per_token : 0;
-    const int h0 = work ? (int)(unit - token * blocks_per_token) * HB : 0;
-    const int heads = p.q_heads + p.kv_heads * (p.append ? 2 : 1);
-    const int D = p.head_dim, e0 = lane * 8;
-    const bool mine = work && e0 < D;
+    const unsigned token = work ? unit / blocks.all : 0, block = work ? unit - token * blocks.all : 0;
     const int pos = __ldg(p.positions + token);
     const bool live = pos >= 0 && pos < p.max_position;
-    const long long cache_row = p.append && h0 + HB > p.q_heads ? rope_cache_row(p, token) : -1;
+    const unsigned b = token / (unsigned)p.tokens, t = token - b * (unsigned)p.tokens;
+    const int D = p.head_dim, half = p.rot_dim / 2;
+    const bool mine = work && lane * 8 < D, turned = lane * 8 < p.rot_dim;
+    const bool halves = !INTERLEAVED && turned;        // this lane's pairs are (first chunk, second chunk)
+    const int e0 = halves ? lane * 4 : lane * 8, e1 = halves ? half + lane * 4 : lane * 8 + 4;
 
-    RopeVec<T> x[HB];
-    RopeRow r[HB];
-#pragma unroll
-    for (int j = 0; j < HB; ++j) {
-        r[j].dst = -1;
-        if (mine && h0 + j < heads) {
-            r[j] = rope_row(p, token, h0 + j, cache_row);
-            if (p.append && r[j].kind != 0 && !live) r[j].dst = -1;
-            x[j].load(rope_src<T>(p, r[j]) + e0);
+    // the block's kind, its heads, where they lie and go
+    const T* src;
+    T* dst;
+    long long step;
+    const void* weight = nullptr;
+    int count;
+    bool goes = true, value = false;
+    if (block < blocks.q) {
+        const int h0 = block * HB;
+        count = p.q_heads - h0;
+        step = p.q_sh;
+        src = static_cast<const T*>(p.q) + b * p.q_sb + t * p.q_st + h0 * step;
+        dst = static_cast<T*>(p.q_out) + ((long long)token * p.q_heads + h0) * D;
+        weight = p.q_weight;
+    } else {
+        value = block >= blocks.q + blocks.k;
+        const int h0 = (block - blocks.q - (value ? blocks.k : 0)) * HB;
+        count = p.kv_heads - h0;
+        step = value ? p.v_sh : p.k_sh;
+        src = value ? static_cast<const T*>(p.v) + b * p.v_sb + t * p.v_st : static_cast<const T*>(p.k) + b * p.k_sb + t * p.k_st;
+        src += h0 * step;
+        weight = value ? nullptr : p.k_weight;
+        if (p.append) {
+            const long long row = live ? rope_cache_row(p, token) : -1;
+            goes = row >= 0;
+            dst = static_cast<T*>(value ? p.v_cache : p.k_cache) + row + (long long)h0 * D;
+        } else {
+            dst = static_cast<T*>(p.k_out) + ((long long)token * p.kv_heads + h0) * D;
         }
     }
-    // angles of this lane's elements; beyond rot_dim (and for padding) cosine 1, sine 0
-    const int half = p.rot_dim / 2;
-    const bool turned = mine && e0 < p.rot_dim;
-    float c[8], s[8];
-    if (h0 < p.q_heads + p.kv_heads) {
-        const float* cs = p.cos_sin + (long long)(live ? pos : 0) * p.rot_dim;
-        if constexpr (INTERLEAVED) {
-            float4 a = make_float4(1.f, 1.f, 1.f, 1.f), b = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (turned && live) {
-                a = __ldg(reinterpret_cast<const float4*>(cs + e0 / 2));
-                b = __ldg(reinterpret_cast<const float4*>(cs + half + e0 / 2));
-            }
-            c[0] = c[1] = a.x; c[2] = c[3] = a.y; c[4] = c[5] = a.z; c[6] = c[7] = a.w;
-            s[1] = b.x; s[3] = b.y; s[5] = b.z; s[7] = b.w;
-            s[0] = -b.x; s[2] = -b.y; s[4] = -b.z; s[6] = -b.w;
-        } else {
-            const int i0 = e0 < half ? e0 : e0 - half;
-            float4 a[2] = {make_float4(1.f, 1.f, 1.f, 1.f), make_float4(1.f, 1.f, 1.f, 1.f)};
-            float4 b[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
-            if (turned && live) {
+    RopeVec<T> x[HB];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    a[i] = __ldg(reinterpret_cast<const float4*>(cs + i0) + i);
-                    b[i] = __ldg(reinterpret_cast<const float4*>(cs + half + i0) + i);
+    for (int j = 0; j < HB; ++j)
+        if (mine && j < count) x[j].load(src + j * step, e0, e1);
+    float w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 1.f;
+    if (weight && mine) {
+        if (p.weight_f32) {
+            RopeVec<float> f;
+            f.load(static_cast<const float*>(weight), e0, e1);
+            f.get(w);
+        } else {
+            RopeVec<T> f;
+            f.load(static_cast<const T*>(weight), e0, e1);
+            f.get(w);
+        }
+    }
+    // the angles of this lane's four pairs
+    float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (mine && turned && live && !value) {
+        const float* at = p.cos_sin + (long long)pos * p.rot_dim + lane * 4;
+        cs = __ldg(reinterpret_cast<const float4*>(at));
+        sn = __ldg(reinterpret_cast<const float4*>(at + half));
+    }
+    const float ca[4] = {cs.x, cs.y, cs.z, cs.w}, sa[4] = {sn.x, sn.y, sn.z, sn.w};
+    const float ms[4] = {-sn.x, -sn.y, -sn.z, -sn.w};
+#pragma unroll
+    for (int j = 0; j < HB; ++j) {
+        // (the groups of a warp may have blocks of different kinds: all take part in the shuffles)
+        float v[8];
+        if (mine && j < count) {
+            x[j].get(v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.f;
+        }
+        float rs = 1.f;
+        if (p.q_weight) {
+            float s2[2] = {0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) rope_fma2(s2, v + i, v + i, s2);
+            float ss = s2[0] + s2[1];
+#pragma unroll
+            for (int z = L / 2; z >= 1; z >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, z, L);
+            rs = rsqrtf(ss / (float)D + p.eps);
+        }
+        if (!mine || j >= count || !goes) continue;
+        if (!value) {
+            const float r2[2] = {rs, rs};
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                rope_mul2(y + i, w + i, r2);
+                rope_mul2(v + i, v + i, y + i);
+            }
+            if constexpr (INTERLEAVED) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    y[2 * i] = v[2 * i] * ca[i] - v[2 * i + 1] * sa[i];
+                    y[2 * i + 1] = v[2 * i + 1] * ca[i] + v[2 * i] * sa[i];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    rope_mul2(y + i, v + i + 4, ms + i);
+                    rope_fma2(y + i, v + i, ca + i, y + i);
+                    rope_mul2(y + i + 4, v + i, sa + i);
+                    rope_fma2(y + i + 4, v + i + 4, ca + i, y + i + 4);
                 }
             }
-            const float sign = e0 < half ? -1.f : 1.f;
+            if (!live) {                               // padding: query (and dense key) rows of zeros
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                c[4 * i] = a[i].x; c[4 * i + 1] = a[i].y; c[4 * i + 2] = a[i].z; c[4 * i + 3] = a[i].w;
-                s[4 * i] = sign * b[i].x; s[4 * i + 1] = sign * b[i].y; s[4 * i + 2] = sign * b[i].z; s[4 * i + 3] = sign * b[i].w;
+                for (int i = 0; i < 8; ++i) y[i] = 0.f;
             }
+            x[j].set(y);
         }
-    }
-    const bool norm = p.q_weight != nullptr;
-    const int partner = turned ? (e0 < half ? lane + half / 8 : lane - half / 8) : lane;
-#pragma unroll
-    for (int j = 0; j < HB; ++j) {
-        const int kind = h0 + j < p.q_heads ? 0 : h0 + j < p.q_heads + p.kv_heads ? 1 : 2;
-        // (the heads of a warp's groups may differ in kind: every lane takes part in the shuffles)
-        float v[8], ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-        const bool row = mine && h0 + j < heads;
-        if (row) x[j].get(v);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(v[i], v[i], ss);
-#pragma unroll
-        for (int z = L / 2; z >= 1; z >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, z, L);
-        const float rs = norm ? rsqrtf(ss / (float)D + p.eps) : 1.f;
-        if (row && norm && kind != 2) {
-            const void* w = kind == 0 ? p.q_weight : p.k_weight;
-            float wf[8];
-            if (p.weight_f32) {
-                RopeVec<float> t;
-                t.load(static_cast<const float*>(w) + e0);
-                t.get(wf);
-            } else {
-                RopeVec<T> t;
-                t.load(static_cast<const T*>(w) + e0);
-                t.get(wf);
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] *= rs * wf[i];
-        }
-        float o[8];
-        if constexpr (INTERLEAVED) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = v[i ^ 1];
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = __shfl_sync(0xffffffffu, v[i], partner, L);
-        }
-        if (row && r[j].dst >= 0) {
-            if (kind != 2) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = live ? fmaf(v[i], c[i], o[i] * s[i]) : 0.f;
-                x[j].set(v);
-            }
-            x[j].store(rope_dst<T>(p, r[j]) + e0);
-        }
+        x[j].store(dst + j * D, e0, e1);
     }
 }
 

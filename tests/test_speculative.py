@@ -16,6 +16,7 @@ Tolerances.  h(t) is half a step of a type relative to the value: finfo(t).eps /
   the fp32 terms.  A forgotten or wrongly seen key among L changes it by about 1/sqrt(L).
 """
 
+import ctypes
 import math
 
 import pytest
@@ -554,7 +555,7 @@ def test_c_entry_points_refuse_bad_arguments():
     assert ws(2, 4, 8, 2, 128, 16, 64) > 0 and ws(2, 65, 8, 2, 128, 16, 64) == 0 and ws(0, 4, 8, 2, 128, 16, 64) == 0
     assert ws(64, 8, 32, 8, 128, 16, 256) % 256 == 0
 
-    strides = attn.speculative._Strides(*([128] * 9))
+    strides = (ctypes.c_int64 * 9)(*([128] * 9))
 
     def rope(dtype=2, wdtype=2, b=2, t=3, hq=8, hkv=2, d=128, rot=128, eps=1e-6, k_out=one, cache=None, st=strides, qw=one,
              kw=one, slots=one, maxpos=10):
