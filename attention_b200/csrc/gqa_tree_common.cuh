@@ -76,46 +76,62 @@ __device__ __forceinline__ long long tree_phys_row(const TreeParams& p, const in
 }
 
 // Where a run begins: `b` the sequence that holds its first tile, `first` that tile's number in the
-// sequence, `count` tiles in all.
+// sequence, `count` tiles in all; `len` and `drafts` of b.  `empties`: some sequence has no key.
 struct TreeRun {
-    int b, first;
+    int b, first, len, drafts;
     long long count;
+    bool empties;
 };
 
 // Run `r` (all threads of the CTA call it).  s_scan: NT / 32 + 4 words of 8 bytes.
 template <int NT>
 __device__ __forceinline__ TreeRun tree_find_run(const TreeParams& p, int r, long long* s_scan) {
     constexpr int NW = NT / 32;
+    constexpr long long kEmpty = 1ll << 62;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int len = 0, drafts = 0;
+    bool empties = false;
     // inclusive prefix of the tiles of NT sequences from b0 on; the chunk's total in `sum`
-    auto scan = [&](int b0, long long& incl, long long& mine, long long& sum) {
-        mine = b0 + tid < p.batch ? tree_tiles(tree_len(p, b0 + tid)) : 0;
+    auto scan = [&](int b0, long long& incl, int& mine, long long& sum) {
+        const bool in = b0 + tid < p.batch;
+        len = in ? tree_len(p, b0 + tid) : 0;
+        drafts = in ? tree_drafts(p, b0 + tid) : 0;
+        mine = tree_tiles(len);
         incl = mine;
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) {
             const long long up = __shfl_up_sync(0xffffffffu, incl, s);
             if (lane >= s) incl += up;
         }
+        const bool none = __any_sync(0xffffffffu, in && len == 0);
         __syncthreads();
-        if (lane == 31) s_scan[warp] = incl;
+        if (lane == 31) s_scan[warp] = incl | (none ? kEmpty : 0);
         __syncthreads();
         sum = 0;
         long long before = 0;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
             const long long x = s_scan[w];
-            if (w < warp) before += x;
-            sum += x;
+            empties |= (x & kEmpty) != 0;
+            if (w < warp) before += x & ~kEmpty;
+            sum += x & ~kEmpty;
         }
         incl += before;
     };
-    long long incl, mine, sum, total = 0;
+    long long incl, sum, total = 0;
+    int mine;
     for (int b0 = 0; b0 < p.batch; b0 += NT) {
         scan(b0, incl, mine, sum);
         total += sum;
     }
-    const long long start = total * r / p.n_ranges;
-    const long long end = total * (r + 1) / p.n_ranges;
+    long long start, end;
+    if (total < (1 << 20) && p.n_ranges <= 4000) {     // (a 32-bit division is a good deal shorter)
+        start = (unsigned)total * (unsigned)r / (unsigned)p.n_ranges;
+        end = (unsigned)total * (unsigned)(r + 1) / (unsigned)p.n_ranges;
+    } else {
+        start = total * r / p.n_ranges;
+        end = total * (r + 1) / p.n_ranges;
+    }
     TreeRun run;
     run.count = end - start;
     if (tid == 0) { s_scan[NW] = p.batch; s_scan[NW + 1] = 0; }
@@ -127,6 +143,8 @@ __device__ __forceinline__ TreeRun tree_find_run(const TreeParams& p, int r, lon
         if (mine > 0 && start >= lo && start < base + incl) {
             s_scan[NW] = b0 + tid;
             s_scan[NW + 1] = start - lo;
+            s_scan[NW + 2] = len;
+            s_scan[NW + 3] = drafts;
         }
         base += sum;
         if (base > start) break;
@@ -134,6 +152,9 @@ __device__ __forceinline__ TreeRun tree_find_run(const TreeParams& p, int r, lon
     __syncthreads();
     run.b = (int)s_scan[NW];
     run.first = (int)s_scan[NW + 1];
+    run.len = (int)s_scan[NW + 2];
+    run.drafts = (int)s_scan[NW + 3];
+    run.empties = empties;
     return run;
 }
 
@@ -162,113 +183,138 @@ __device__ __forceinline__ long long tree_part_row(const TreeParams& p, int slot
 // Merge: CTA column x stands for the boundary between runs x and x + 1.  If it is the first
 // boundary inside a sequence, the CTA joins that sequence's partials, in run order.
 //   M = max m_r,  out = sum 2^(m_r - M) acc_r / sum 2^(m_r - M) l_r
-// One warp per row.  Lane i looks after piece i of a round of 32 (its maximum, sum and weight), then
-// the warp adds the pieces' rows four at a time, so that a long sequence's many pieces cost a few
-// round trips to memory and not two each (17 pieces x 256 rows: 29 us one after the other).
+// Lane i of a warp looks after run r0 + i (where it begins; the row's maximum, sum and weight there), so
+// that a long sequence's many pieces cost a few round trips to memory and not some each; then the warp
+// adds the pieces' rows, kTreeMergeRows rows by four pieces at a time.
 // VEC: D is a multiple of 4, a lane owns columns 4 lane .. 4 lane + 3 (and + 128).
 // ---------------------------------------------------------------------------
 constexpr int kTreeMergeWarps = 8;
+constexpr int kTreeMergeRows = 2;                    // rows of a warp at a time
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kTreeMergeWarps * 32) gqa_tree_merge_kernel(const TreeParams p) {
     pdl_launch_dependents();
     pdl_wait();
+    constexpr unsigned ALL = 0xffffffffu;
     const int r0 = blockIdx.x;                       // last run before the boundary
-    const int4 here = __ldcg(p.info + r0 + 1);
-    const int4 prev = __ldcg(p.info + r0);
-    if (here.x >= p.batch || here.y == 0) return;    // no tile behind it, or between two sequences
-    if (prev.x == here.x && prev.y != 0) return;     // an earlier boundary is inside this sequence too
-    const int b = here.x;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int slot0 = 2 * r0 + (prev.x == b ? 0 : 1);   // the first piece; every later one begins its run
-    int r1 = r0;                                     // last run that holds a piece of b
-    for (;;) {
-        const int r = r1 + 1 + lane;
-        const bool in = r < p.n_ranges && __ldcg(p.info + r).x == b;
-        const unsigned inside = __ballot_sync(0xffffffffu, in);
-        if (inside == 0xffffffffu) { r1 += 32; continue; }
-        r1 += __ffs(~inside) - 1;
-        break;
-    }
+    const int4 mine = __ldcg(p.info + min(r0 + lane, p.n_ranges - 1));
+    const int b = __shfl_sync(ALL, mine.x, 1), first = __shfl_sync(ALL, mine.y, 1);
+    const int prev_b = __shfl_sync(ALL, mine.x, 0), prev_first = __shfl_sync(ALL, mine.y, 0);
+    if (b >= p.batch || first == 0) return;          // no tile behind it, or between two sequences
+    if (prev_b == b && prev_first != 0) return;      // an earlier boundary is inside this sequence too
+    const int slot0 = 2 * r0 + (prev_b == b ? 0 : 1);   // the first piece; every later one begins its run
+    // a run whose first tile is b's holds a piece of it, if it has a tile at all (.z)
+    auto inside = [&](int q0, int4 info) {
+        const int r = q0 + lane;
+        return r < p.n_ranges && (r == r0 || info.x == b);
+    };
     const int n_rows = p.rows * p.kv_heads;
     const int D = p.head_dim;
     constexpr int NV = VEC ? 2 : 8;                  // groups of columns of a lane
     constexpr int W = VEC ? 4 : 1;                   // columns of a group
-    for (int row = blockIdx.y * kTreeMergeWarps + warp; row < n_rows; row += gridDim.y * kTreeMergeWarps) {
-        const int kvh = row / p.rows, rr = row - kvh * p.rows;
-        float acc[NV][W], sum = 0.f, mx = -INFINITY;
+    constexpr int RW = VEC ? kTreeMergeRows : 1;
+    const int step = gridDim.y * kTreeMergeWarps * RW;
+    for (int row0 = (blockIdx.y * kTreeMergeWarps + warp) * RW; row0 < n_rows; row0 += step) {
+        float acc[RW][NV][W], sum[RW], mx[RW];
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int c = 0; c < W; ++c) acc[j][c] = 0.f;
-        for (int q0 = r0; q0 <= r1; q0 += 32) {
-            const int r = q0 + lane;
-            long long at = 0;
-            float2 ml = make_float2(-INFINITY, 0.f);
-            if (r <= r1 && __ldcg(p.info + r).z) {   // (a run without a tile has no piece)
-                at = tree_part_row(p, r == r0 ? slot0 : 2 * r, kvh, rr);
-                ml = __ldcg(p.part_ml + at);
-            }
-            const bool use = ml.y != 0.f;            // it saw something (NaN counts)
-            float m = use ? ml.x : -INFINITY;
-#pragma unroll
-            for (int x = 16; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-            const unsigned live = __ballot_sync(0xffffffffu, use);
-            if (live == 0) continue;
-            const float mn = fmaxf(mx, m);
-            const float alpha = mx == -INFINITY ? 0.f : fast_exp2(mx - mn);
-            mx = mn;
-            const float w = use ? fast_exp2(ml.x - mn) : 0.f;
-            float s = use ? w * ml.y : 0.f;
-#pragma unroll
-            for (int x = 16; x >= 1; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-            sum = sum * alpha + s;
+        for (int k = 0; k < RW; ++k) {
+            sum[k] = 0.f;
+            mx[k] = -INFINITY;
 #pragma unroll
             for (int j = 0; j < NV; ++j)
 #pragma unroll
-                for (int c = 0; c < W; ++c) acc[j][c] *= alpha;
-            for (unsigned todo = live; todo;) {
-                float x[4][NV][W], wt[4];
+                for (int c = 0; c < W; ++c) acc[k][j][c] = 0.f;
+        }
+        for (int q0 = r0; q0 < p.n_ranges; q0 += 32) {
+            const int4 info = q0 == r0 ? mine : __ldcg(p.info + min(q0 + lane, p.n_ranges - 1));
+            const bool in = inside(q0, info), has = in && info.z != 0;
+            const unsigned last_in = __ballot_sync(ALL, in) >> 31;
+            const int slot = q0 + lane == r0 ? slot0 : 2 * (q0 + lane);
+            // (rows of one kv head or of two: the row number runs on over the heads)
+            const long long at = (long long)slot * n_rows + row0;
+            float w[RW];
+            unsigned live[RW], any = 0;
+#pragma unroll
+            for (int k = 0; k < RW; ++k) {
+                float2 ml = make_float2(-INFINITY, 0.f);
+                if (has && row0 + k < n_rows) ml = __ldcg(p.part_ml + at + k);
+                const bool use = ml.y != 0.f;        // it saw something (NaN counts)
+                float m = use ? ml.x : -INFINITY;
+#pragma unroll
+                for (int x = 16; x >= 1; x >>= 1) m = fmaxf(m, __shfl_xor_sync(ALL, m, x));
+                live[k] = __ballot_sync(ALL, use);
+                any |= live[k];
+                const float mn = fmaxf(mx[k], m);
+                const float alpha = mx[k] == -INFINITY ? 0.f : fast_exp2(mx[k] - mn);
+                mx[k] = mn;
+                w[k] = use ? fast_exp2(ml.x - mn) : 0.f;
+                float s = use ? w[k] * ml.y : 0.f;
+#pragma unroll
+                for (int x = 16; x >= 1; x >>= 1) s += __shfl_xor_sync(ALL, s, x);
+                sum[k] = sum[k] * alpha + s;
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+#pragma unroll
+                    for (int c = 0; c < W; ++c) acc[k][j][c] *= alpha;
+            }
+            for (unsigned todo = any; todo;) {
+                float x[4][RW][NV][W];
+                int from[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    const int from = todo ? __ffs(todo) - 1 : 0;
-                    const bool has = todo != 0;
+                    from[u] = todo ? __ffs(todo) - 1 : -1;
                     todo &= todo - 1;
-                    wt[u] = __shfl_sync(0xffffffffu, w, from);
-                    const float* src = p.part_acc + __shfl_sync(0xffffffffu, at, from) * D;
+                    const long long src = __shfl_sync(ALL, at, from[u] & 31);
 #pragma unroll
-                    for (int j = 0; j < NV; ++j) {
-                        const int c = W * (lane + 32 * j);
-                        if (!has || c >= D) {
+                    for (int k = 0; k < RW; ++k) {
+                        // (a piece that saw nothing may hold anything)
+                        const bool load = from[u] >= 0 && (live[k] >> (from[u] & 31) & 1u);
 #pragma unroll
-                            for (int i = 0; i < W; ++i) x[u][j][i] = 0.f;
-                            continue;
-                        }
-                        if constexpr (VEC) {
-                            const float4 t = __ldcg(reinterpret_cast<const float4*>(src + c));
-                            x[u][j][0] = t.x; x[u][j][1] = t.y; x[u][j][2] = t.z; x[u][j][3] = t.w;
-                        } else {
-                            x[u][j][0] = __ldcg(src + c);
+                        for (int j = 0; j < NV; ++j) {
+                            const int c = W * (lane + 32 * j);
+                            if (!load || c >= D) {
+#pragma unroll
+                                for (int i = 0; i < W; ++i) x[u][k][j][i] = 0.f;
+                                continue;
+                            }
+                            if constexpr (VEC) {
+                                const float4 t = __ldcg(reinterpret_cast<const float4*>(p.part_acc + (src + k) * D + c));
+                                x[u][k][j][0] = t.x; x[u][k][j][1] = t.y; x[u][k][j][2] = t.z; x[u][k][j][3] = t.w;
+                            } else {
+                                x[u][k][j][0] = __ldcg(p.part_acc + (src + k) * D + c);
+                            }
                         }
                     }
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
 #pragma unroll
-                    for (int j = 0; j < NV; ++j)
+                    for (int k = 0; k < RW; ++k) {
+                        const float wt = __shfl_sync(ALL, w[k], from[u] & 31);
 #pragma unroll
-                        for (int c = 0; c < W; ++c) acc[j][c] = fmaf(wt[u], x[u][j][c], acc[j][c]);
+                        for (int j = 0; j < NV; ++j)
+#pragma unroll
+                            for (int c = 0; c < W; ++c) acc[k][j][c] = fmaf(wt, x[u][k][j][c], acc[k][j][c]);
+                    }
             }
+            if (!last_in) break;                     // the sequence ends within these runs
         }
-        const int tok = rr / p.group, head = kvh * p.group + rr - tok * p.group;
-        T* dst = static_cast<T*>(p.out) + (((long long)b * p.tokens + tok) * p.q_heads + head) * D;
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int k = 0; k < RW; ++k) {
+            const int row = row0 + k;
+            if (row >= n_rows) continue;
+            const int kvh = row / p.rows, rr = row - kvh * p.rows;
+            const int tok = rr / p.group, head = kvh * p.group + rr - tok * p.group;
+            T* dst = static_cast<T*>(p.out) + (((long long)b * p.tokens + tok) * p.q_heads + head) * D;
+            const float inv = sum[k] == 0.f ? 0.f : 1.f / sum[k];
 #pragma unroll
-            for (int i = 0; i < W; ++i) {
-                const int c = W * (lane + 32 * j) + i;
-                if (c < D) dst[c] = from_f32<T>(sum == 0.f ? 0.f : acc[j][i] * inv);
-            }
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    const int c = W * (lane + 32 * j) + i;
+                    if (c < D) dst[c] = from_f32<T>(sum[k] == 0.f ? 0.f : acc[k][j][i] * inv);
+                }
+        }
     }
 }
 

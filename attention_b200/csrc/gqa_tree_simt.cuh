@@ -85,8 +85,8 @@ __global__ void __launch_bounds__(kTreeSimtThreads) gqa_tree_simt_kernel(const T
     const T* kp = static_cast<const T*>(p.k) + (long long)kvh * D;
     const T* vp = static_cast<const T*>(p.v) + (long long)kvh * D;
 
-    tree_zero_empty<T>(p);
     const TreeRun run = tree_find_run<kTreeSimtThreads>(p, run_no, s_scan);
+    if (run.empties) tree_zero_empty<T>(p);
     if (unit == 0) tree_publish(p, run_no, run);
     long long left = run.count;
     int first = run.first;

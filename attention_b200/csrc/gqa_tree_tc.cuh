@@ -103,6 +103,20 @@ __device__ __forceinline__ void tree_tma_load(uint32_t dst, const CUtensorMap* m
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
         ::"r"(dst), "l"(map), "r"(x), "r"(head), "r"(y), "r"(bar) : "memory");
 }
+__device__ __forceinline__ void tree_prefetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+// two lanes of packed fp32: d = a * b + c, d = a * b
+__device__ __forceinline__ void tree_fma2(float& d0, float& d1, float a0, float a1, float b, float c0, float c1) {
+    asm("{\n\t.reg .b64 ra, rb, rc;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %4};\n\tmov.b64 rc, {%5, %6};\n\t"
+        "fma.rn.f32x2 ra, ra, rb, rc;\n\tmov.b64 {%0, %1}, ra;\n\t}"
+        : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void tree_mul2(float& d0, float& d1, float a0, float a1, float b) {
+    asm("{\n\t.reg .b64 ra, rb;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %4};\n\t"
+        "mul.rn.f32x2 ra, ra, rb;\n\tmov.b64 {%0, %1}, ra;\n\t}"
+        : "=f"(d0), "=f"(d1) : "f"(a0), "f"(a1), "f"(b));
+}
 // an arrival with the bytes that TMA copies will bring
 __device__ __forceinline__ void mbar_arrive_tx(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -186,6 +200,11 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
         for (int i = 0; i < kTreeBadRing; ++i) s_bad[i] = 0ull;
         s_dead = 0;
     }
+    if (TMA && warp == 4 * NX && lane == 0) {        // the loader warp: the maps' first use is not to wait for them
+        tree_prefetch_map(&map_q);
+        tree_prefetch_map(&map_k);
+        tree_prefetch_map(&map_v);
+    }
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
@@ -193,8 +212,8 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
 
     pdl_launch_dependents();
     pdl_wait();
-    tree_zero_empty<T>(p);
     const TreeRun run = tree_find_run<NT>(p, run_no, s_scan);
+    if (run.empties) tree_zero_empty<T>(p);
     if (unit == 0) tree_publish(p, run_no, run);
     // A wait that runs out ends this warp's work: it starts no copy or product any more (but keeps its
     // barriers with other warps), the others follow at their next wait.  The status word: 2, the
@@ -248,15 +267,18 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
     const int row = row0 + (MODE == 2 ? X * p.tile_rows : 0) + quad * 32 + lane;   // softmax threads
     const int tok = row / p.group;
     const bool has_row = quad * 32 + lane < p.tile_rows && row < p.rows;   // (else a dead lane of a live warp)
-    int len = 0, nd = 0, len_next = 0, nd_next = 0;
+    int len = 0, nd = 0, len_next = run.len, nd_next = run.drafts;
     unsigned long long word = 0ull, word_next = 0ull;
+    auto ask_word = [&](int b) {
+        if (is_softmax && p.mask && has_row) word_next = __ldg(p.mask + (long long)b * p.tokens + tok);
+    };
     auto ask_sequence = [&](int b) {
         if (b >= p.batch) return;
         len_next = tree_len(p, b);
         nd_next = tree_drafts(p, b);
-        if (is_softmax && p.mask && has_row) word_next = __ldg(p.mask + (long long)b * p.tokens + tok);
+        ask_word(b);
     };
-    if (left > 0) ask_sequence(run.b);
+    if (left > 0) ask_word(run.b);
     for (int b = run.b; left > 0 && b < p.batch; ++b, first = 0) {
         len = len_next;
         nd = nd_next;
@@ -290,6 +312,16 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                     return lane < boxes && pg <= last_page ? __ldg(table + pg) : 0;
                 };
                 int id = ask(t0);
+                auto load_q = [&]() {
+                    const int box_tok = min(p.tokens, p.tile_rows / p.group);
+                    if (lane == 0) mbar_arrive_tx(q_full, (uint32_t)(tiles_live * KB * box_tok * p.group * 128));
+                    __syncwarp();
+                    if (lane < tiles_live * KB)
+                        tree_tma_load_q(sq + lane / KB * G::kQBytes + lane % KB * (BM * 128), &map_q, lane % KB * 64, kvh,
+                                        b * p.tokens + (row0 + lane / KB * p.tile_rows) / p.group, q_full);
+                    __syncwarp();
+                };
+                if (lw == 1 && piece == 0) load_q();
                 for (int j = 0; j < n; ++j) {
                     const int J = J0 + j, t = t0 + j * BN, use = J / stages, stage = J - use * stages;
                     const int pg = page_of(t);
@@ -305,17 +337,11 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                     if (mine) tree_tma_load(ring + stage * G::kTileBytes + my_off, map, my_col * 64, kvh, y, landed);
                     if (j + 1 < n) id = ask(t + BN);
                     __syncwarp();
-                    if (lw == 1 && j == 0) {
+                    if (lw == 1 && j == 0 && piece > 0) {
                         // (the rings have room for that tile whatever becomes of this piece's queries)
-                        if (piece >= 1) wait_bar(q_empty, (piece - 1) & 1);
+                        wait_bar(q_empty, (piece - 1) & 1);
                         if (!alive) break;
-                        const int box_tok = min(p.tokens, p.tile_rows / p.group);
-                        if (lane == 0) mbar_arrive_tx(q_full, (uint32_t)(tiles_live * KB * box_tok * p.group * 128));
-                        __syncwarp();
-                        if (lane < tiles_live * KB)
-                            tree_tma_load_q(sq + lane / KB * G::kQBytes + lane % KB * (BM * 128), &map_q, lane % KB * 64, kvh,
-                                            b * p.tokens + (row0 + lane / KB * p.tile_rows) / p.group, q_full);
-                        __syncwarp();
+                        load_q();
                     }
                 }
             } else {
@@ -551,21 +577,23 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                         wait_bar(v_full + (MODE == 1 ? X * NSV + stage : stage) * 8, v_parity);
                         const uint32_t tile = sv + stage * G::kTileBytes;
                         const int live_warps = X ? warps_b : warps_a;
+                        const int from = max(0, off), end = min(HN, max(t1 - t_base, from)), by = live_warps * RPI;
 #pragma unroll 4
-                        for (int r = max(0, off) + quad * RPI + ld_row0; r < HN; r += live_warps * RPI) {
+                        for (int r = from + quad * RPI + ld_row0; r < end; r += by) {
                             const uint32_t at = chunk_addr(tile, h * HN + r, BN);
-                            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                            bool store = true;
-                            if (t_base + r < t1) {
-                                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                             : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
-                                store = clean(x);
-                                if (store) atomicOr(&s_bad[piece % kTreeBadRing], 1ull << (t_base + r - prefix));
-                            }
-                            if (store)
+                            uint4 x;
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                         : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
+                            if (clean(x)) {
+                                atomicOr(&s_bad[piece % kTreeBadRing], 1ull << (t_base + r - prefix));
                                 asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w)
                                              : "memory");
+                            }
                         }
+#pragma unroll 4
+                        for (int r = end + quad * RPI + ld_row0; r < HN; r += by)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(chunk_addr(tile, h * HN + r, BN)), "r"(0u)
+                                         : "memory");
                         tc::fence_async_smem();
                         __syncwarp();
                     }
@@ -603,6 +631,8 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
             const unsigned long long seen_bad = bits & *reinterpret_cast<volatile unsigned long long*>(&s_bad[piece % kTreeBadRing]);
             const bool write = has_row && alive;
             const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+            if (whole) { w_own *= inv; w_other *= inv; }         // (a partial stays unnormalised)
+            const bool plain = __all_sync(0xffffffffu, use_own && use_other);
             const long long at = tree_part_row(p, 2 * run_no + (b == run.b ? 0 : 1), kvh, row);
             if (write && !whole && (MODE != 1 || X == 0)) p.part_ml[at] = make_float2(m_all, l_all);
             T* dst = static_cast<T*>(p.out) + (((long long)b * p.tokens + tok) * p.q_heads + kvh * p.group + row - tok * p.group) * D;
@@ -610,24 +640,34 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
 #pragma unroll
             for (int cc = 0; cc < COLS; cc += 32) {
                 const int c0 = cc + (MODE == 1 ? X * COLS : 0);
-                uint32_t o[32];
+                uint32_t raw[32];
+                float o[32];
                 __syncwarp();
-                tc::tmem_ld32(o_addr + c0, o);
-                if constexpr (MODE == 1) {
-                    uint32_t o2[32];
-                    tc::tmem_ld32(tmem + G::kColO + (X ^ 1) * DP + lane_sel + c0, o2);
+                tc::tmem_ld32(o_addr + c0, raw);
+                if constexpr (MODE != 1) {
                     tc::tmem_ld_wait();
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        const float a = use_own ? __uint_as_float(o[c]) * w_own : 0.f;
-                        const float e = use_other ? __uint_as_float(o2[c]) * w_other : 0.f;
-                        o[c] = __float_as_uint(a + e);
-                    }
-                } else {
-                    tc::tmem_ld_wait();
+                    for (int c = 0; c < 32; c += 2)
+                        tree_mul2(o[c], o[c + 1], __uint_as_float(raw[c]), __uint_as_float(raw[c + 1]), w_own);
                     if (!use_own) {
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) o[c] = 0u;
+                        for (int c = 0; c < 32; ++c) o[c] = 0.f;
+                    }
+                } else {
+                    uint32_t raw2[32];
+                    tc::tmem_ld32(tmem + G::kColO + (X ^ 1) * DP + lane_sel + c0, raw2);
+                    tc::tmem_ld_wait();
+                    if (!plain) {                                // some row saw nothing in one of the chains
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) {
+                            if (!use_own) raw[c] = 0u;
+                            if (!use_other) raw2[c] = 0u;
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2) {
+                        tree_mul2(o[c], o[c + 1], __uint_as_float(raw[c]), __uint_as_float(raw[c + 1]), w_own);
+                        tree_fma2(o[c], o[c + 1], __uint_as_float(raw2[c]), __uint_as_float(raw2[c + 1]), w_other, o[c], o[c + 1]);
                     }
                 }
                 if (!write || c0 >= D) continue;
@@ -639,7 +679,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                     for (int c = 0; c < 32; ++c) {
                         if (c0 + c >= D) continue;
                         const float val = to_f32<T>(vr[c]);
-                        if ((__float_as_uint(val) & 0x7f800000u) == 0x7f800000u) o[c] = __float_as_uint(__uint_as_float(o[c]) + val);
+                        if ((__float_as_uint(val) & 0x7f800000u) == 0x7f800000u) o[c] += val;
                     }
                 }
                 if (whole) {
@@ -647,17 +687,17 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                     for (int c8 = 0; c8 < 4; ++c8) {
                         if (c0 + c8 * 8 >= D) continue;
                         uint4 v;
-                        v.x = Ops::pack(__uint_as_float(o[c8 * 8 + 0]) * inv, __uint_as_float(o[c8 * 8 + 1]) * inv);
-                        v.y = Ops::pack(__uint_as_float(o[c8 * 8 + 2]) * inv, __uint_as_float(o[c8 * 8 + 3]) * inv);
-                        v.z = Ops::pack(__uint_as_float(o[c8 * 8 + 4]) * inv, __uint_as_float(o[c8 * 8 + 5]) * inv);
-                        v.w = Ops::pack(__uint_as_float(o[c8 * 8 + 6]) * inv, __uint_as_float(o[c8 * 8 + 7]) * inv);
+                        v.x = Ops::pack(o[c8 * 8 + 0], o[c8 * 8 + 1]);
+                        v.y = Ops::pack(o[c8 * 8 + 2], o[c8 * 8 + 3]);
+                        v.z = Ops::pack(o[c8 * 8 + 4], o[c8 * 8 + 5]);
+                        v.w = Ops::pack(o[c8 * 8 + 6], o[c8 * 8 + 7]);
                         *reinterpret_cast<uint4*>(dst + c0 + c8 * 8) = v;
                     }
                 } else {
-                    uint4* acc = reinterpret_cast<uint4*>(p.part_acc + at * D + c0);
+                    float4* acc = reinterpret_cast<float4*>(p.part_acc + at * D + c0);
 #pragma unroll
                     for (int c4 = 0; c4 < 8; ++c4)
-                        if (c0 + c4 * 4 < D) acc[c4] = make_uint4(o[c4 * 4], o[c4 * 4 + 1], o[c4 * 4 + 2], o[c4 * 4 + 3]);
+                        if (c0 + c4 * 4 < D) acc[c4] = make_float4(o[c4 * 4], o[c4 * 4 + 1], o[c4 * 4 + 2], o[c4 * 4 + 3]);
                 }
             }
             __syncwarp();

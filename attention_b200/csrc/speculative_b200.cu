@@ -288,7 +288,8 @@ cudaError_t launch_tree(const TreeParams& p, const TreePlan& t, bool tc, const T
     }
     if (e != cudaSuccess || t.n_runs == 1) return e;
     const int rows = p.rows * p.kv_heads;
-    const int by = std::min((rows + kTreeMergeWarps - 1) / kTreeMergeWarps, 65535);
+    const int per_cta = kTreeMergeWarps * kTreeMergeRows;
+    const int by = std::min((rows + per_cta - 1) / per_cta, 65535);
     auto merge = p.head_dim % 4 == 0 ? gqa_tree_merge_kernel<T, true> : gqa_tree_merge_kernel<T, false>;
     return launch_pdl(merge, dim3((unsigned)(t.n_runs - 1), (unsigned)by), kTreeMergeWarps * 32, 0, stream, p);
 }

@@ -161,8 +161,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, *, eps=1e-6, inte
         _validate_rope(q, k, q_weight, k_weight, cos_sin, positions, eps)
         raise RuntimeError("invalid qk_norm_rope arguments")   # not reached: the line above raises
     if q_out is None and k_out is None:
-        q_out = torch.empty(qs, dtype=q.dtype, device=q.device)
-        k_out = torch.empty(ks, dtype=q.dtype, device=q.device)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     else:
         both = (q, k, q_weight, k_weight, cos_sin, positions)
         q_out = _check_out(q_out, q, "q_out", both)
@@ -242,7 +242,7 @@ def qk_norm_rope_append(q, k, v, q_weight, k_weight, cos_sin, positions, k_cache
         _validate_append(q, k, v, k_cache, v_cache, block_table, slots, positions)
         raise RuntimeError("invalid qk_norm_rope_append arguments")   # not reached: the lines above raise
     if out is None:
-        out = torch.empty(qs, dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
         out = _check_out(out, q, "out", (q, k, v, q_weight, k_weight, cos_sin, positions, slots, k_cache, v_cache,
                                          block_table))
@@ -360,7 +360,7 @@ def gqa_tree_decode(q, k_cache, v_cache, block_table, context_lens, tree_mask=No
         raise ValueError("kernel must be auto, simt or tcgen05")
     device = q.device
     if out is None:
-        out = torch.empty(qs, dtype=q.dtype, device=device)
+        out = torch.empty_like(q)
     else:
         _check_cuda_contiguous(out, "out")
         _check(out.shape == qs and out.dtype == q.dtype and out.device == device, "out must match q")
