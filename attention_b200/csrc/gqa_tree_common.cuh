@@ -7,7 +7,7 @@
 // For one kv head the queries are R = tokens * group rows (row r = token r / group, head r % group)
 // that all read the same keys, so K and V are read once per block of rows.
 //
-// How the work is cut.  The 128-key tiles of all sequences, laid end to end, are cut into
+// How the work is cut.  The tiles (128 keys, or 64) of all sequences, laid end to end, are cut into
 // `n_ranges` equal runs; a run is worked on by one CTA for every (kv head, block of rows), with the
 // kv head fastest in the CTA number so that CTAs side by side read neighbouring bytes of the same
 // pages.  Every CTA derives its run from context_lens itself (nothing is read on the host, no plan
@@ -21,7 +21,8 @@
 
 namespace gqa_b200 {
 
-constexpr int kTreeTile = 128;          // keys of a tile, the unit of the cut
+constexpr int kTreeTile = 128;          // keys of a tile, the unit of the cut (tensor-core kernel)
+constexpr int kTreeSimtTile = 64;       // the same for the CUDA-core kernel: short contexts fill more SMs
 constexpr int kTreeMaxTokens = 64;      // drafted tokens per sequence: bits of a mask word
 
 struct TreeParams {
@@ -64,7 +65,7 @@ __device__ __forceinline__ unsigned long long tree_bits(const TreeParams& p, int
     if (i >= n) return 0ull;
     return tree_bits_of(p, p.mask ? __ldg(p.mask + (long long)b * p.tokens + i) : 0ull, i, n);
 }
-__device__ __forceinline__ int tree_tiles(int len) { return (int)(((long long)len + kTreeTile - 1) / kTreeTile); }
+__device__ __forceinline__ int tree_tiles(int len, int tile) { return (int)(((unsigned)len + (unsigned)tile - 1u) / (unsigned)tile); }
 // Physical row (page * block_size + slot) of a position, the page id clamped into the pool.
 __device__ __forceinline__ long long tree_phys_row(const TreeParams& p, const int32_t* table_row, int t) {
     int page, slot;
@@ -84,7 +85,7 @@ struct TreeRun {
 };
 
 // Run `r` (all threads of the CTA call it).  s_scan: NT / 32 + 4 words of 8 bytes.
-template <int NT>
+template <int NT, int TILE>
 __device__ __forceinline__ TreeRun tree_find_run(const TreeParams& p, int r, long long* s_scan) {
     constexpr int NW = NT / 32;
     constexpr long long kEmpty = 1ll << 62;
@@ -96,7 +97,7 @@ __device__ __forceinline__ TreeRun tree_find_run(const TreeParams& p, int r, lon
         const bool in = b0 + tid < p.batch;
         len = in ? tree_len(p, b0 + tid) : 0;
         drafts = in ? tree_drafts(p, b0 + tid) : 0;
-        mine = tree_tiles(len);
+        mine = tree_tiles(len, TILE);
         incl = mine;
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) {
@@ -186,11 +187,11 @@ __device__ __forceinline__ long long tree_part_row(const TreeParams& p, int slot
 // Lane i of a warp looks after run r0 + i (where it begins; the row's maximum, sum and weight there), so
 // that a long sequence's many pieces cost a few round trips to memory and not some each; then the warp
 // adds the pieces' rows, kTreeMergeRows rows by four pieces at a time.
-// VEC: D is a multiple of 4, a lane owns columns 4 lane .. 4 lane + 3 (and + 128).
+// NV4 > 0: D is a multiple of 4 and at most 128 NV4, a lane owns columns 4 lane .. 4 lane + 3 (and + 128).
 // ---------------------------------------------------------------------------
 constexpr int kTreeMergeWarps = 8;
 constexpr int kTreeMergeRows = 2;                    // rows of a warp at a time
-template <typename T, bool VEC>
+template <typename T, int NV4>
 __global__ void __launch_bounds__(kTreeMergeWarps * 32) gqa_tree_merge_kernel(const TreeParams p) {
     pdl_launch_dependents();
     pdl_wait();
@@ -210,7 +211,8 @@ __global__ void __launch_bounds__(kTreeMergeWarps * 32) gqa_tree_merge_kernel(co
     };
     const int n_rows = p.rows * p.kv_heads;
     const int D = p.head_dim;
-    constexpr int NV = VEC ? 2 : 8;                  // groups of columns of a lane
+    constexpr bool VEC = NV4 > 0;
+    constexpr int NV = VEC ? NV4 : 8;                // groups of columns of a lane
     constexpr int W = VEC ? 4 : 1;                   // columns of a group
     constexpr int RW = VEC ? kTreeMergeRows : 1;
     const int step = gridDim.y * kTreeMergeWarps * RW;

@@ -27,33 +27,34 @@ template <int RB, int DC> struct TreeSimtGeom {
     static_assert(kLX <= 32 && kLK >= 1, "a row pair sits in one warp");
 };
 
-// `n` rows of D elements to shared memory as fp32, columns up to DC and rows whose offset is
-// negative as zeros.
-template <typename T, int DC>
-__device__ __forceinline__ void tree_stage_rows(float* dst, int stride, const T* base, const long long* s_off, int n,
-                                                int D, bool vec) {
-    constexpr int V = 16 / (int)sizeof(T);
+// N rows of D elements to shared memory as fp32, columns up to DC and rows whose offset is negative as
+// zeros.  All of a thread's loads are under way before the first is stored (one after the other, 16
+// round trips per 32 keys made most of the kernel's time).
+template <typename T, int DC, int N>
+__device__ __forceinline__ void tree_stage_rows(float* dst, int stride, const T* base, const long long* s_off, int D, bool vec) {
+    constexpr int V = 16 / (int)sizeof(T), C = DC / V;
     if (vec) {
-        constexpr int C = DC / V;
-        for (int i = threadIdx.x; i < n * C; i += kTreeSimtThreads) {
-            const int r = i / C, c = (i - r * C) * V;
-            float x[V];
-            const long long off = s_off[r];
-            if (off >= 0 && c < D) {
-                const uint4 raw = __ldg(reinterpret_cast<const uint4*>(base + off + c));
-                const T* e = reinterpret_cast<const T*>(&raw);
+        constexpr int PER = (N * C + kTreeSimtThreads - 1) / kTreeSimtThreads;
+        uint4 raw[PER];
 #pragma unroll
-                for (int j = 0; j < V; ++j) x[j] = to_f32<T>(e[j]);
-            } else {
+        for (int k = 0; k < PER; ++k) {
+            const int i = threadIdx.x + k * kTreeSimtThreads, r = i / C, c = (i - r * C) * V;
+            raw[k] = make_uint4(0u, 0u, 0u, 0u);
+            if (i < N * C && c < D && s_off[r] >= 0) raw[k] = __ldg(reinterpret_cast<const uint4*>(base + s_off[r] + c));
+        }
 #pragma unroll
-                for (int j = 0; j < V; ++j) x[j] = 0.f;
-            }
+        for (int k = 0; k < PER; ++k) {
+            const int i = threadIdx.x + k * kTreeSimtThreads, r = i / C, c = (i - r * C) * V;
+            if (i >= N * C) continue;
+            const T* e = reinterpret_cast<const T*>(&raw[k]);
 #pragma unroll
             for (int j = 0; j < V; j += 4)
-                *reinterpret_cast<float4*>(dst + r * stride + c + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+                *reinterpret_cast<float4*>(dst + r * stride + c + j) =
+                    make_float4(to_f32<T>(e[j]), to_f32<T>(e[j + 1]), to_f32<T>(e[j + 2]), to_f32<T>(e[j + 3]));
         }
     } else {
-        for (int i = threadIdx.x; i < n * DC; i += kTreeSimtThreads) {
+#pragma unroll 8
+        for (int i = threadIdx.x; i < N * DC; i += kTreeSimtThreads) {
             const int r = i / DC, c = i - r * DC;
             const long long off = s_off[r];
             dst[r * stride + c] = off >= 0 && c < D ? to_f32<T>(base[off + c]) : 0.f;
@@ -85,19 +86,19 @@ __global__ void __launch_bounds__(kTreeSimtThreads) gqa_tree_simt_kernel(const T
     const T* kp = static_cast<const T*>(p.k) + (long long)kvh * D;
     const T* vp = static_cast<const T*>(p.v) + (long long)kvh * D;
 
-    const TreeRun run = tree_find_run<kTreeSimtThreads>(p, run_no, s_scan);
+    const TreeRun run = tree_find_run<kTreeSimtThreads, kTreeSimtTile>(p, run_no, s_scan);
     if (run.empties) tree_zero_empty<T>(p);
     if (unit == 0) tree_publish(p, run_no, run);
     long long left = run.count;
     int first = run.first;
     for (int b = run.b; left > 0 && b < p.batch; ++b, first = 0) {
         const int len = tree_len(p, b);
-        const int tiles = tree_tiles(len);
+        const int tiles = tree_tiles(len, kTreeSimtTile);
         if (tiles == 0) continue;
         const int take = (int)(left < tiles - first ? left : tiles - first);
         left -= take;
         const bool whole = take == tiles;
-        const int t0 = first * kTreeTile, t1 = min(len, (first + take) * kTreeTile);
+        const int t0 = first * kTreeSimtTile, t1 = min(len, (first + take) * kTreeSimtTile);
         const int n = tree_drafts(p, b), prefix = len - n;
         const int32_t* table = p.table + (long long)b * p.max_pages;
 
@@ -108,7 +109,7 @@ __global__ void __launch_bounds__(kTreeSimtThreads) gqa_tree_simt_kernel(const T
                                       : -1;
         }
         __syncthreads();
-        tree_stage_rows<T, DC>(s_q, ST, qp, s_off, RB, D, vec);
+        tree_stage_rows<T, DC, RB>(s_q, ST, qp, s_off, D, vec);
 
         unsigned long long bits[2];
         bool live[2];
@@ -131,8 +132,8 @@ __global__ void __launch_bounds__(kTreeSimtThreads) gqa_tree_simt_kernel(const T
             if (tid < KN)
                 s_off[tid] = t + tid < t1 ? tree_phys_row(p, table, t + tid) * p.kv_heads * D : -1;
             __syncthreads();
-            tree_stage_rows<T, DC>(s_k, ST, kp, s_off, KN, D, vec);
-            tree_stage_rows<T, DC>(s_v, ST, vp, s_off, KN, D, vec);
+            tree_stage_rows<T, DC, KN>(s_k, ST, kp, s_off, D, vec);
+            tree_stage_rows<T, DC, KN>(s_v, ST, vp, s_off, D, vec);
             __syncthreads();
             float s[2][LK];
 #pragma unroll

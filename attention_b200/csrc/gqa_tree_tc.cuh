@@ -212,7 +212,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
 
     pdl_launch_dependents();
     pdl_wait();
-    const TreeRun run = tree_find_run<NT>(p, run_no, s_scan);
+    const TreeRun run = tree_find_run<NT, kTreeTile>(p, run_no, s_scan);
     if (run.empties) tree_zero_empty<T>(p);
     if (unit == 0) tree_publish(p, run_no, run);
     // A wait that runs out ends this warp's work: it starts no copy or product any more (but keeps its
@@ -284,7 +284,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
         nd = nd_next;
         word = word_next;
         ask_sequence(b + 1);
-        const int tiles = tree_tiles(len);
+        const int tiles = tree_tiles(len, kTreeTile);
         if (tiles == 0) continue;
         const int take = min(left, tiles - first);
         left -= take;

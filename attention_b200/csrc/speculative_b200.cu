@@ -104,19 +104,20 @@ struct TreePlan {
     int row_block, row_blocks, n_runs;
     long long units;
 };
-TreePlan tree_plan(int batch, int tokens, int q_heads, int kv_heads, long long cap_tokens, int row_block, int ctas_per_sm) {
+TreePlan tree_plan(int batch, int tokens, int q_heads, int kv_heads, long long cap_tokens, int row_block, int ctas_per_sm,
+                   int tile) {
     TreePlan t;
     const long long rows = (long long)tokens * (q_heads / kv_heads);
     t.row_block = row_block;
     t.row_blocks = (int)((rows + row_block - 1) / row_block);
     t.units = (long long)kv_heads * t.row_blocks;
-    const long long cap_tiles = (long long)batch * ((cap_tokens + kTreeTile - 1) / kTreeTile);
+    const long long cap_tiles = (long long)batch * ((cap_tokens + tile - 1) / tile);
     t.n_runs = tree_run_count(t.units, (long long)kSms * ctas_per_sm, cap_tiles);
     return t;
 }
 TreePlan tree_plan_simt(int batch, int tokens, int q_heads, int kv_heads, long long cap_tokens) {
     return tree_plan(batch, tokens, q_heads, kv_heads, cap_tokens, tree_simt_rows(tokens * (q_heads / kv_heads)),
-                     kTreeSimtCtasPerSm);
+                     kTreeSimtCtasPerSm, kTreeSimtTile);
 }
 
 
@@ -140,7 +141,7 @@ int tree_tile_rows(int group) { return group <= kTreeBM ? kTreeBM / group * grou
 TreePlan tree_plan_tc(int batch, int tokens, int q_heads, int kv_heads, int head_dim, long long cap_tokens, bool tma) {
     const int group = q_heads / kv_heads, tile = tree_tile_rows(group);
     const int tiles = tma && head_dim <= 128 && tokens * group > tile ? 2 : 1;
-    return tree_plan(batch, tokens, q_heads, kv_heads, cap_tokens, tile * tiles, 1);
+    return tree_plan(batch, tokens, q_heads, kv_heads, cap_tokens, tile * tiles, 1, kTreeTile);
 }
 
 // Status word of the tensor-core kernel: 0 ok, 2 = a bounded wait ran out, 3 = the dynamic shared
@@ -290,7 +291,9 @@ cudaError_t launch_tree(const TreeParams& p, const TreePlan& t, bool tc, const T
     const int rows = p.rows * p.kv_heads;
     const int per_cta = kTreeMergeWarps * kTreeMergeRows;
     const int by = std::min((rows + per_cta - 1) / per_cta, 65535);
-    auto merge = p.head_dim % 4 == 0 ? gqa_tree_merge_kernel<T, true> : gqa_tree_merge_kernel<T, false>;
+    auto merge = p.head_dim % 4 != 0 ? gqa_tree_merge_kernel<T, 0>
+                 : p.head_dim <= 128 ? gqa_tree_merge_kernel<T, 1>
+                                     : gqa_tree_merge_kernel<T, 2>;
     return launch_pdl(merge, dim3((unsigned)(t.n_runs - 1), (unsigned)by), kTreeMergeWarps * 32, 0, stream, p);
 }
 
@@ -457,10 +460,12 @@ int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache
                      tree_maps(&maps, dtype == GQA_B200_BF16, p);
     const TreePlan plan = tc ? tree_plan_tc(batch, tokens, q_heads, kv_heads, head_dim, cap, tma)
                              : tree_plan_simt(batch, tokens, q_heads, kv_heads, cap);
-    const long long cap_tiles = (long long)batch * ((cap + kTreeTile - 1) / kTreeTile);
+    const long long cap_tiles = (long long)batch * ((cap + kTreeSimtTile - 1) / kTreeSimtTile);
     if (plan.n_runs * plan.units > kIntMax || cap_tiles / plan.n_runs >= kIntMax / 2) return GQA_B200_ERR_INT32_RANGE;
     const TreeScratch lay = tree_scratch(plan, tokens, q_heads, head_dim);
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < lay.total)
+    // (the published size, whichever kernel runs)
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) ||
+        workspace_bytes < gqa_b200_tree_workspace_bytes(batch, tokens, q_heads, kv_heads, head_dim, block_size, max_pages))
         return GQA_B200_ERR_WORKSPACE;
     char* ws = static_cast<char*>(workspace);
     p.info = reinterpret_cast<int4*>(ws + lay.info);
