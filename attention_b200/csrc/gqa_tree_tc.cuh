@@ -210,7 +210,6 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
     tc::tc_fence_after();
     const uint32_t tmem = s_tmem;
 
-    pdl_launch_dependents();
     pdl_wait();
     const TreeRun run = tree_find_run<NT, kTreeTile>(p, run_no, s_scan);
     if (run.empties) tree_zero_empty<T>(p);
@@ -709,6 +708,9 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
         J0 += n;
         ++piece;
     }
+    // (not earlier: the merge kernel's CTAs, and behind them the next call's, would take their places on
+    // the SMs in an order of chance; 138 against 127 us on the batch of 64 x 8 tokens, call after call)
+    pdl_launch_dependents();
     if (is_load) cp_async_wait<0>();
     tc::tc_fence_before();
     __syncthreads();
