@@ -160,6 +160,12 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
     const int warps_a = (min(rows_here, p.tile_rows) + 31) / 32; // live softmax warps of chain A, of B
     const int warps_b = MODE == 1 ? warps_a : tiles_live > 1 ? (rows_here - p.tile_rows + 31) / 32 : 0;
     const int D = p.head_dim;
+    // Up to 32 rows fill one softmax warp per chain, and both would sit on one scheduler (a warp reaches the
+    // tensor-memory lanes of its number mod 4 only).  So the rows lie in the query tile twice, at 0 and at
+    // 64, and chain B takes its scores and sums from lanes 64 .. 95.  What the chains exchange at the end of
+    // a piece then goes through shared memory: the query tile's rows 32 .. 63 and 96 .. 127, which nobody needs.
+    const bool spread = MODE == 1 && TMA && rows_here <= 32;
+    const int home = spread ? 2 * X : 0;             // first lane quadrant of this chain's rows
 
     const uint32_t s_base = tc::smem_u32(smem);
     if (s_base & 1023u) {                            // the swizzled tiles need a 1024-byte aligned base
@@ -263,9 +269,10 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
     int left = (int)run.count;                       // (fits: the launcher checks it)
     int first = run.first;
     // what a piece needs of its sequence is asked for a piece ahead
-    const int row = row0 + (MODE == 2 ? X * p.tile_rows : 0) + quad * 32 + lane;   // softmax threads
+    const int wq = quad - home;                                  // softmax warps: number among those of the chain
+    const int row_l = wq * 32 + lane, row = row0 + (MODE == 2 ? X * p.tile_rows : 0) + row_l;
     const int tok = row / p.group;
-    const bool has_row = quad * 32 + lane < p.tile_rows && row < p.rows;   // (else a dead lane of a live warp)
+    const bool has_row = row_l >= 0 && row_l < p.tile_rows && row < p.rows;   // (else a dead lane, or warp)
     int len = 0, nd = 0, len_next = run.len, nd_next = run.drafts;
     unsigned long long word = 0ull, word_next = 0ull;
     auto ask_word = [&](int b) {
@@ -313,11 +320,13 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                 int id = ask(t0);
                 auto load_q = [&]() {
                     const int box_tok = min(p.tokens, p.tile_rows / p.group);
-                    if (lane == 0) mbar_arrive_tx(q_full, (uint32_t)(tiles_live * KB * box_tok * p.group * 128));
+                    const int copies = spread ? 2 : tiles_live;
+                    if (lane == 0) mbar_arrive_tx(q_full, (uint32_t)(copies * KB * box_tok * p.group * 128));
                     __syncwarp();
-                    if (lane < tiles_live * KB)
-                        tree_tma_load_q(sq + lane / KB * G::kQBytes + lane % KB * (BM * 128), &map_q, lane % KB * 64, kvh,
-                                        b * p.tokens + (row0 + lane / KB * p.tile_rows) / p.group, q_full);
+                    if (lane < copies * KB)
+                        tree_tma_load_q(sq + lane / KB * (spread ? 64 * 128 : G::kQBytes) + lane % KB * (BM * 128), &map_q,
+                                        lane % KB * 64, kvh,
+                                        b * p.tokens + (row0 + (spread ? 0 : lane / KB * p.tile_rows)) / p.group, q_full);
                     __syncwarp();
                 };
                 if (lw == 1 && piece == 0) load_q();
@@ -478,7 +487,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                 }
             }
             __syncwarp();
-        } else if (quad < (X ? warps_b : warps_a)) {
+        } else if (wq >= 0 && wq < (X ? warps_b : warps_a)) {
             // =============================== softmax warps of chain X ===============================
             const int prefix = len - nd;
             const bool live = has_row && tok < nd;
@@ -510,7 +519,9 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                         for (int c = 0; c < 32; ++c) sc[q * 32 + c] = __uint_as_float(r[c]);
                     }
                     const int off = prefix - t_base;             // where the drafted tokens begin in this half
-                    if (!live || off < HN) {                     // (t1 <= len: no key is missing before them)
+                    // (t1 <= len: no key is missing before them.  A dead lane's scores of other halves may be
+                    // anything: it leaves its sums out in the end.)
+                    if (off < HN) {
                         unsigned long long w = 0ull;             // bit c: key t_base + c is visible
                         if (live) {
                             if (off >= 64) w = ~0ull;
@@ -534,7 +545,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                         a1 = tc::max3(a1, sc[HN - 2], sc[HN - 1]);
                         mx = fmaxf(tc::max3(a0, a1, a2), a3) * p.scale_log2;
                     }
-                    const bool need = mx > m_run + kRescaleSlack;
+                    const bool need = live && mx > m_run + kRescaleSlack;
                     float alpha = 1.f;
                     if (need) {
                         const float mn = fmaxf(m_run, mx);
@@ -578,7 +589,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                         const int live_warps = X ? warps_b : warps_a;
                         const int from = max(0, off), end = min(HN, max(t1 - t_base, from)), by = live_warps * RPI;
 #pragma unroll 4
-                        for (int r = from + quad * RPI + ld_row0; r < end; r += by) {
+                        for (int r = from + wq * RPI + ld_row0; r < end; r += by) {
                             const uint32_t at = chunk_addr(tile, h * HN + r, BN);
                             uint4 x;
                             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
@@ -590,7 +601,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                             }
                         }
 #pragma unroll 4
-                        for (int r = end + quad * RPI + ld_row0; r < HN; r += by)
+                        for (int r = end + wq * RPI + ld_row0; r < HN; r += by)
                             asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(chunk_addr(tile, h * HN + r, BN)), "r"(0u)
                                          : "memory");
                         tc::fence_async_smem();
@@ -603,6 +614,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                 }
             }
 
+            if (!live) { m_run = -INFINITY; l_run = 0.f; }
             // ---- the piece's rows: to `out` when it is the whole sequence, else as a partial ----
             if (nx > 0) {
                 wait_bar(bar_o + (X * 2 + 1) * 8, (c0 + nx - 1) & 1);
@@ -612,13 +624,30 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
             // A chain without a visible key (or a tile) has sum 0; its O may hold anything and is left out.
             float m_all = m_run, l_all = l_run, w_own = 1.f, w_other = 0.f;
             bool use_own = l_run != 0.f, use_other = false;
+            constexpr int COLS = MODE == 1 ? DP / 2 : DP;        // columns this warp stores
+            // spread: 4 KB for 32 columns of chain x, element (column, lane)
+            auto exchange = [&](int x, int cc) {
+                const int i = x * (COLS / 32) + cc / 32;
+                return sq + (i >> 1) * (BM * 128) + 32 * 128 + (i & 1) * (64 * 128) + lane * 4;
+            };
             if constexpr (MODE == 1) {
-                s_ml[X * BM + quad * 32 + lane] = make_float2(m_run, l_run);
+                s_ml[X * BM + row_l] = make_float2(m_run, l_run);
                 __syncwarp();
+                if (spread) {                                    // the columns that the other warp stores
+#pragma unroll
+                    for (int cc = 0; cc < COLS; cc += 32) {
+                        uint32_t o[32];
+                        tc::tmem_ld32(o_addr + (X ^ 1) * COLS + cc, o);
+                        tc::tmem_ld_wait();
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            asm volatile("st.shared.b32 [%0], %1;" ::"r"(exchange(X, cc) + c * 128), "r"(o[c]) : "memory");
+                    }
+                }
                 tc::tc_fence_before();
-                asm volatile("bar.sync %0, 64;" ::"r"(quad + 1) : "memory");
+                asm volatile("bar.sync %0, 64;" ::"r"(wq + 1) : "memory");
                 tc::tc_fence_after();
-                const float2 other = s_ml[(X ^ 1) * BM + quad * 32 + lane];
+                const float2 other = s_ml[(X ^ 1) * BM + row_l];
                 use_other = other.y != 0.f;
                 m_all = fmaxf(use_own ? m_run : -INFINITY, use_other ? other.x : -INFINITY);
                 w_own = use_own ? fast_exp2(m_run - m_all) : 0.f;
@@ -635,7 +664,6 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
             const long long at = tree_part_row(p, 2 * run_no + (b == run.b ? 0 : 1), kvh, row);
             if (write && !whole && (MODE != 1 || X == 0)) p.part_ml[at] = make_float2(m_all, l_all);
             T* dst = static_cast<T*>(p.out) + (((long long)b * p.tokens + tok) * p.q_heads + kvh * p.group + row - tok * p.group) * D;
-            constexpr int COLS = MODE == 1 ? DP / 2 : DP;        // columns this warp stores
 #pragma unroll
             for (int cc = 0; cc < COLS; cc += 32) {
                 const int c0 = cc + (MODE == 1 ? X * COLS : 0);
@@ -654,7 +682,13 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                     }
                 } else {
                     uint32_t raw2[32];
-                    tc::tmem_ld32(tmem + G::kColO + (X ^ 1) * DP + lane_sel + c0, raw2);
+                    if (spread) {
+#pragma unroll
+                        for (int c = 0; c < 32; ++c)
+                            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(raw2[c]) : "r"(exchange(X ^ 1, cc) + c * 128) : "memory");
+                    } else {
+                        tc::tmem_ld32(tmem + G::kColO + (X ^ 1) * DP + lane_sel + c0, raw2);
+                    }
                     tc::tmem_ld_wait();
                     if (!plain) {                                // some row saw nothing in one of the chains
 #pragma unroll
@@ -701,7 +735,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
             }
             __syncwarp();
             tc::tc_fence_before();                   // the loads of O are done before this warp's next arrival
-            if constexpr (MODE == 1) asm volatile("bar.sync %0, 64;" ::"r"(quad + 1) : "memory");   // ... and the other warp's
+            if constexpr (MODE == 1) asm volatile("bar.sync %0, 64;" ::"r"(wq + 1) : "memory");   // ... and the other warp's
         }
         C0[0] += tiles_of(0);
         C0[1] += tiles_of(1);
