@@ -67,6 +67,10 @@
 
 namespace gqa_b200 {
 
+// Status word: 0 ok, 2 (| barrier << 8 | warp << 16) = a bounded wait ran out, 3 = the dynamic shared
+// memory base was not 1024-byte aligned.
+static __device__ int g_tree_tc_status;
+
 constexpr int kTreeBM = 128;            // rows of a query tile
 constexpr int kTreeTmemCols = 512;
 
@@ -129,7 +133,7 @@ constexpr int kTreeBadRing = 16;
 template <typename T, int DP, int MODE, bool TMA>
 __global__ void __launch_bounds__(kTreeTcWarps<MODE, TMA> * 32, 1)
 gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                   const __grid_constant__ CUtensorMap map_v, int* status) {
+                   const __grid_constant__ CUtensorMap map_v) {
     using G = TreeTcGeom<DP, MODE>;
     using Ops = MmaOps<T>;
     constexpr int BM = kTreeBM, BN = G::kBN, HN = G::kHN, NSK = G::kStagesK, NSV = G::kStagesV, KB = G::kKB;
@@ -169,7 +173,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
 
     const uint32_t s_base = tc::smem_u32(smem);
     if (s_base & 1023u) {                            // the swizzled tiles need a 1024-byte aligned base
-        if (tid == 0) atomicExch(status, 3);
+        if (tid == 0) atomicExch(&g_tree_tc_status, 3);
         return;
     }
     const uint32_t sq = s_base, sk = s_base + G::kOffK, sv = s_base + G::kOffV;
@@ -230,7 +234,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
         if (alive && !tc::mbar_wait(bar, parity, dead ? 1000ull : 1000000000ull)) {
             *reinterpret_cast<volatile int*>(&s_dead) = 1;
             alive = false;
-            if (!dead) atomicCAS(status, 0, 2 | (int)((bar - q_full) >> 3) << 8 | warp << 16);
+            if (!dead) atomicCAS(&g_tree_tc_status, 0, 2 | (int)((bar - q_full) >> 3) << 8 | warp << 16);
         }
     };
 

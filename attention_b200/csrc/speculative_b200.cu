@@ -22,7 +22,6 @@
 namespace gqa_b200 {
 namespace {
 
-constexpr int kMaxDevices = 64;
 constexpr int kSms = 148;                    // the cut of the work is for a B200, whatever runs it
 constexpr int kTreeSimtCtasPerSm = 3;
 constexpr long long kIntMax = 0x7fffffffll;
@@ -144,27 +143,6 @@ TreePlan tree_plan_tc(int batch, int tokens, int q_heads, int kv_heads, int head
     return tree_plan(batch, tokens, q_heads, kv_heads, cap_tokens, tile * tiles, 1, kTreeTile);
 }
 
-// Status word of the tensor-core kernel: 0 ok, 2 = a bounded wait ran out, 3 = the dynamic shared
-// memory base was not 1024-byte aligned.  Read with gqa_b200_tree_tc_status.
-__device__ int g_tree_tc_status;
-int* g_tree_tc_status_ptr[kMaxDevices];
-
-cudaError_t tree_tc_status_address(int** out) {
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return e;
-    if (dev < 0 || dev >= kMaxDevices) return cudaErrorInvalidDevice;
-    std::lock_guard<std::mutex> lock(g_mutex);
-    if (!g_tree_tc_status_ptr[dev]) {
-        void* ptr = nullptr;
-        e = cudaGetSymbolAddress(&ptr, g_tree_tc_status);
-        if (e != cudaSuccess) return e;
-        g_tree_tc_status_ptr[dev] = static_cast<int*>(ptr);
-    }
-    *out = g_tree_tc_status_ptr[dev];
-    return cudaSuccess;
-}
-
 struct TreeScratch {
     size_t info, ml, acc, total;
 };
@@ -250,16 +228,13 @@ bool tree_maps(TreeMaps* m, bool bf16, const TreeParams& p) {
 
 template <typename T, int DP, int MODE, bool TMA>
 cudaError_t launch_tree_tc(const TreeParams& p, const TreePlan& t, const TreeMaps& maps, cudaStream_t stream) {
-    int* status = nullptr;
-    cudaError_t e = tree_tc_status_address(&status);
-    if (e != cudaSuccess) return e;
     using G = TreeTcGeom<DP, MODE>;
     static_assert(G::kBN == (DP <= 128 ? 128 : 64), "tree_tc_keys");
     auto kernel = gqa_tree_tc_kernel<T, DP, MODE, TMA>;
-    e = allow_smem(reinterpret_cast<const void*>(kernel), G::kSmemBytes);
+    const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), G::kSmemBytes);
     if (e != cudaSuccess) return e;
     return launch_pdl(kernel, dim3((unsigned)(t.n_runs * t.units)), kTreeTcWarps<MODE, TMA> * 32, G::kSmemBytes, stream, p,
-                      maps.q, maps.k, maps.v, status);
+                      maps.q, maps.k, maps.v);
 }
 template <typename T>
 cudaError_t launch_tree_tc_dim(const TreeParams& p, const TreePlan& t, const TreeMaps* maps, cudaStream_t stream) {
@@ -432,7 +407,7 @@ int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache
     if (num_blocks <= 0 || block_size <= 0) return GQA_B200_ERR_CACHE_SHAPE;
     if (max_pages <= 0) return GQA_B200_ERR_MAX_PAGES;
     if (!(std::isfinite(scale) && scale > 0.f)) return GQA_B200_ERR_SCALE;
-    if (num_blocks > kIntMax || (long long)tokens * q_heads > 65535) return GQA_B200_ERR_INT32_RANGE;
+    if (num_blocks > kIntMax || (long long)tokens * q_heads > (1 << 20)) return GQA_B200_ERR_INT32_RANGE;
     if (kernel != GQA_B200_KERNEL_AUTO && kernel != GQA_B200_KERNEL_SIMT && kernel != GQA_B200_KERNEL_TCGEN05)
         return GQA_B200_ERR_KERNEL;
     if (batch == 0) return GQA_B200_OK;
@@ -482,15 +457,12 @@ int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache
 }
 
 int gqa_b200_tree_tc_status(int reset) {
-    int* status = nullptr;
-    cudaError_t e = tree_tc_status_address(&status);
-    if (e != cudaSuccess) return -(int)e;
     int host = 0;
-    e = cudaMemcpy(&host, status, sizeof(int), cudaMemcpyDeviceToHost);
+    cudaError_t e = cudaMemcpyFromSymbol(&host, g_tree_tc_status, sizeof(int));
     if (e != cudaSuccess) return -(int)e;
     if (reset) {
         const int zero = 0;
-        e = cudaMemcpy(status, &zero, sizeof(int), cudaMemcpyHostToDevice);
+        e = cudaMemcpyToSymbol(g_tree_tc_status, &zero, sizeof(int));
         if (e != cudaSuccess) return -(int)e;
     }
     return host;

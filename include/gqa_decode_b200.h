@@ -323,7 +323,8 @@ GQA_B200_API int gqa_b200_tree_decode(const void* q, const void* k_cache, const 
                                       int max_pages, float scale, int kernel, void* workspace,
                                       size_t workspace_bytes, void* stream);
 
-/* Debug aid for the tcgen05 tree kernel: as gqa_b200_prefill_tc_status. */
+/* Debug aid for the tcgen05 tree kernel: as gqa_b200_prefill_tc_status (the low byte of a
+ * status that is not zero is 2 or 3). */
 GQA_B200_API int gqa_b200_tree_tc_status(int reset);
 
 /* Move rows within sequences: the K and V rows at positions src_positions[b, i]

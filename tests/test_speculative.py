@@ -18,6 +18,9 @@ Tolerances.  h(t) is half a step of a type relative to the value: finfo(t).eps /
 
 import ctypes
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -412,6 +415,104 @@ def test_tree_two_graphs_and_two_streams_share_nothing():
     assert torch.equal(outs[0], attn.gqa_tree_decode(*dcs[0][:6]))
 
 
+@gpu
+@pytest.mark.parametrize("kernel", ["auto", "simt"])
+def test_tree_many_short_and_few_long_pieces_again_and_again(kernel):
+    """Chains of a CTA drift apart over many short sequences; the same bits every time."""
+    gen = torch.Generator().manual_seed(4)
+    for t, hq, hkv, d in [(2, 8, 4, 128), (7, 8, 4, 128), (20, 8, 2, 64), (40, 8, 2, 128)]:
+        lengths = [int(x) for x in torch.randint(t, 700, (90,), generator=gen)]
+        dq, dk, dv, dt, dl, dm, _ = on_gpu(*tree_case(lengths, t, hq, hkv, d, 16, torch.bfloat16, seed=t))
+        want = attn.gqa_tree_decode(dq, dk, dv, dt, dl, dm, kernel=kernel)
+        simt = attn.gqa_tree_decode(dq, dk, dv, dt, dl, dm, kernel="simt")
+        # both kernels within their roundings of the same value (P and the result; A <= max |v|)
+        assert (want.float() - simt.float()).abs().max() <= 3 * half_step(torch.bfloat16) * float(dv.float().abs().max())
+        for _ in range(60):
+            assert torch.equal(attn.gqa_tree_decode(dq, dk, dv, dt, dl, dm, kernel=kernel), want)
+
+
+@gpu
+def test_offsets_beyond_32_bits():
+    """A pool of more than 2^32 bytes per cache and 2^31 elements, pages at its end."""
+    bs, hkv, d, t = 16, 8, 256, 4
+    pool = 2**31 // (bs * hkv * d) + 40
+    gen = torch.Generator().manual_seed(0)
+    kc = torch.empty(pool, bs, hkv, d, dtype=torch.bfloat16, device=DEV)
+    vc = torch.empty_like(kc)
+    lengths = [75, 40]
+    lens = torch.tensor(lengths, dtype=torch.int32)
+    used = 8
+    table = (pool - 1 - torch.arange(2 * used).view(2, used) * 2).to(torch.int32)
+    rows = torch.randn(2, 2 * used, bs, hkv, d, generator=gen).bfloat16()
+    at = table.flatten().long().to(DEV)
+    kc[at], vc[at] = rows[0].to(DEV), rows[1].to(DEV)
+    small = torch.arange(2 * used, dtype=torch.int32).view(2, used)
+    q = torch.randn(2, t, 16, d, generator=gen).bfloat16()
+    for kernel in ("auto", "simt"):
+        got = attn.gqa_tree_decode(*on_gpu(q), kc, vc, *on_gpu(table, lens), kernel=kernel)
+        check_tree(got, (q, rows[0], rows[1], small, lens, None, None))
+    key, val = torch.randn(2, 2, t, hkv, d, generator=gen).bfloat16()
+    slots = torch.tensor([[75, 76, 100, 127], [40, 41, 42, 43]], dtype=torch.int32)
+    cs = rope_table(200, d)
+    dkey = key.to(DEV)
+    attn.qk_norm_rope_append(q.to(DEV), dkey, val.to(DEV), None, None, cs.to(DEV), slots.to(DEV), kc, vc, table.to(DEV))
+    keys = attn.qk_norm_rope(q.to(DEV), dkey, None, None, cs.to(DEV), slots.to(DEV))[1].cpu()
+    live = torch.ones(2, t, dtype=torch.bool)
+    ref.write_rows(rows[0], keys, small, slots, live)
+    ref.write_rows(rows[1], val, small, slots, live)
+    src = torch.tensor([[100, 127, 3], [43, 40, -1]], dtype=torch.int32)
+    dst = torch.tensor([75, 40], dtype=torch.int32)
+    attn.kv_compact(kc, vc, *on_gpu(table, src, dst))
+    want = [ref.compact(r, small, src, dst) for r in rows]
+    assert torch.equal(kc[at].cpu(), want[0]) and torch.equal(vc[at].cpu(), want[1])
+    frm, to = table[0, :3].to(DEV), (table[0, :3] - 1).to(DEV)
+    attn.kv_copy_pages(kc, vc, frm, to)
+    assert torch.equal(kc[to.long()], kc[frm.long()]) and torch.equal(vc[to.long()], vc[frm.long()])
+
+
+@gpu
+def test_first_call_of_a_process_may_be_captured():
+    """Nothing is looked up or set up in a way that a stream capture forbids."""
+    code = """
+import sys
+sys.path.insert(0, {root!r})
+import torch
+import attention_b200 as attn
+q = torch.randn(2, 4, 8, 128, device="cuda").bfloat16()
+kc = torch.randn(9, 16, 2, 128, device="cuda").bfloat16()
+vc = torch.randn_like(kc)
+table = torch.arange(8, device="cuda", dtype=torch.int32).view(2, 4)
+lens = torch.tensor([60, 33], device="cuda", dtype=torch.int32)
+cs = torch.randn(64, 128, device="cuda")
+pos = torch.tensor([[3, 4, 5, 6], [7, 8, 9, 10]], device="cuda", dtype=torch.int32)
+pages = torch.tensor([[0], [8]], device="cuda", dtype=torch.int32)
+def step():
+    r = attn.qk_norm_rope_append(q, q[:, :, :2], q[:, :, 2:4], None, None, cs, pos, kc, vc, table)
+    out = attn.gqa_tree_decode(r, kc, vc, table, lens)
+    slow = attn.gqa_tree_decode(r, kc, vc, table, lens, kernel="simt")
+    attn.kv_compact(kc, vc, table, pos, lens - 4)
+    attn.kv_copy_pages(kc, vc, pages[0], pages[1])
+    return r, out, slow
+torch.cuda.synchronize()
+keep = kc.clone(), vc.clone()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = step()
+g.replay()
+torch.cuda.synchronize()
+got = [x.clone() for x in (*got, kc, vc)]
+kc.copy_(keep[0]); vc.copy_(keep[1])
+want = [*step(), kc, vc]
+assert all(torch.equal(a, b) for a, b in zip(got, want))
+assert attn.speculative.tree_tc_status() == 0
+del g
+print("captured")
+"""
+    root = str(Path(__file__).resolve().parents[1])
+    run = subprocess.run([sys.executable, "-c", code.format(root=root)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "captured" in run.stdout, run.stderr[-2000:]
+
+
 # --------------------------------------------------------------------------- moves in the cache
 @gpu
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -617,6 +718,8 @@ def test_front_doors_refuse_bad_tensors():
                                  draft_lens=a["drafts"])
     with pytest.raises(ValueError):
         attn.gqa_tree_decode(q, k, v, table, lens, mask, kernel="mma")
+    with pytest.raises(RuntimeError, match="cannot run"):       # float32 has the CUDA-core kernel only
+        attn.gqa_tree_decode(q.float(), k.float(), v.float(), table, lens, mask, kernel="tcgen05")
 
     cs = rope_table(16, 64).to(DEV)
     pos = torch.zeros(2, 4, dtype=torch.int32, device=DEV)
