@@ -82,9 +82,12 @@ cudaError_t allow_smem(const void* kernel, size_t smem) {
 // tree attention
 // ---------------------------------------------------------------------------
 // Number of runs the tiles are cut into for `units` CTAs per run on `slots` resident CTAs: as many
-// as fill the GPU once, or up to four times if that leaves fewer CTAs idle in the last round (a
-// single round of 4 runs x 32 kv heads would leave 20 of 148 SMs without work; two rounds of 288
-// CTAs leave 8 of 296).
+// as fill the GPU once, or up to four times if that leaves far fewer CTAs idle in the last round
+// (80 units: one round uses 80 of 148 SMs, two use 240 of 296).  A round more has to give an eighth of
+// the GPU: memory is busy with four fifths of the SMs at work already, and each round ends in pieces
+// of its own.  About 80 000 keys x kv heads of D 128, 1 / 2 / 3 or 4 rounds: 20 kv heads (140, 140,
+// 148 SMs of 148 at work) 127 / - / 147 us, 32 (128, 144) 126 / 130 / -, 40 (120, 140) 123 / 127 / -,
+// 64 (128, 128, 144) 129 / - / 150.
 int tree_run_count(long long units, long long slots, long long cap_tiles) {
     long long best = 1;
     double best_fill = 0.0;
@@ -92,7 +95,7 @@ int tree_run_count(long long units, long long slots, long long cap_tiles) {
         const long long n = slots * rounds / units;
         if (n < 1) continue;
         const double fill = (double)(n * units) / (double)(slots * rounds);
-        if (fill > best_fill + 0.03) { best_fill = fill; best = n; }
+        if (fill > best_fill + 0.12) { best_fill = fill; best = n; }
     }
     return (int)std::max(1ll, std::min(best, cap_tiles));
 }
