@@ -47,14 +47,11 @@ struct TreeParams {
     float scale_log2;
 };
 
-__device__ __forceinline__ int tree_len(const TreeParams& p, int b) {
-    const int len = __ldg(p.lens + b);
-    return len < 0 ? 0 : (len > p.cap_tokens ? p.cap_tokens : len);
-}
+__device__ __forceinline__ int tree_clamp(int n, int top) { return n < 0 ? 0 : (n > top ? top : n); }
+__device__ __forceinline__ int tree_len(const TreeParams& p, int b) { return tree_clamp(__ldg(p.lens + b), p.cap_tokens); }
 __device__ __forceinline__ int tree_drafts(const TreeParams& p, int b) {
     if (!p.draft_lens) return p.tokens;
-    const int n = __ldg(p.draft_lens + b);
-    return n < 0 ? 0 : (n > p.tokens ? p.tokens : n);
+    return tree_clamp(__ldg(p.draft_lens + b), p.tokens);
 }
 // Drafted tokens (bits 0 .. n - 1) that row token i < n may see; `word` is its mask word.
 __device__ __forceinline__ unsigned long long tree_bits_of(const TreeParams& p, unsigned long long word, int i, int n) {

@@ -53,6 +53,13 @@
 // what is not finite becomes zero in shared memory and is remembered by token (a row that sees such a
 // token adds the value to its sums when it stores them), rows behind the end become zero.
 //
+// Instruction fetch.  What runs once in a piece is straight-line code that the loop over tiles has pushed
+// out of the instruction caches, and a miss behind the K and V tiles in flight costs 1000 clocks or
+// more: the end of a piece took 8000 clocks and its way to the next piece's first scores 6000, whatever
+// the rows.  So loops over columns stay rolled there, the rare additions of hidden values have a loop
+// of their own, and a chain's two halves share one body (MODE 2, bound by that body, has two):
+// 129 -> 117 us on the batch of 64 x 8 tokens, 45 -> 37 us on a ragged one of 32 x 16 tokens.
+//
 // Precision: scores and sums in fp32, P rounded to the element type (relative error half a step of
 // each probability, as in the other tensor-core kernels), O in fp32.
 #pragma once
@@ -109,6 +116,18 @@ __device__ __forceinline__ void tree_tma_load(uint32_t dst, const CUtensorMap* m
 }
 __device__ __forceinline__ void tree_prefetch_map(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
+// Loads that start where they are written: the compiler moves a plain one down to where its value is used,
+// and behind the K and V tiles in flight a read of HBM takes up to 7000 clocks.
+__device__ __forceinline__ int tree_ask(const int32_t* at) {
+    int x;
+    asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(x) : "l"(at));
+    return x;
+}
+__device__ __forceinline__ unsigned long long tree_ask(const unsigned long long* at) {
+    unsigned long long x;
+    asm volatile("ld.global.nc.b64 %0, [%1];" : "=l"(x) : "l"(at));
+    return x;
 }
 // two lanes of packed fp32: d = a * b + c, d = a * b
 __device__ __forceinline__ void tree_fma2(float& d0, float& d1, float a0, float a1, float b, float c0, float c1) {
@@ -277,21 +296,22 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
     const int row_l = wq * 32 + lane, row = row0 + (MODE == 2 ? X * p.tile_rows : 0) + row_l;
     const int tok = row / p.group;
     const bool has_row = row_l >= 0 && row_l < p.tile_rows && row < p.rows;   // (else a dead lane, or warp)
+    // (as it was loaded: nothing is computed from it, and so waited for, before its piece begins)
     int len = 0, nd = 0, len_next = run.len, nd_next = run.drafts;
     unsigned long long word = 0ull, word_next = 0ull;
     auto ask_word = [&](int b) {
-        if (is_softmax && p.mask && has_row) word_next = __ldg(p.mask + (long long)b * p.tokens + tok);
+        if (is_softmax && p.mask && has_row) word_next = tree_ask(p.mask + (long long)b * p.tokens + tok);
     };
     auto ask_sequence = [&](int b) {
         if (b >= p.batch) return;
-        len_next = tree_len(p, b);
-        nd_next = tree_drafts(p, b);
+        len_next = tree_ask(p.lens + b);
+        if (p.draft_lens) nd_next = tree_ask(p.draft_lens + b);
         ask_word(b);
     };
     if (left > 0) ask_word(run.b);
     for (int b = run.b; left > 0 && b < p.batch; ++b, first = 0) {
-        len = len_next;
-        nd = nd_next;
+        len = tree_clamp(len_next, p.cap_tokens);
+        nd = tree_clamp(nd_next, p.tokens);
         word = word_next;
         ask_sequence(b + 1);
         const int tiles = tree_tiles(len, kTreeTile);
@@ -319,7 +339,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                 const uint32_t my_off = my_col * (BN * 128) + my_page * (box_rows * 128);
                 auto ask = [&](int t) {
                     const int pg = page_of(t) + my_page;
-                    return lane < boxes && pg <= last_page ? __ldg(table + pg) : 0;
+                    return lane < boxes && pg <= last_page ? tree_ask(table + pg) : 0;
                 };
                 int id = ask(t0);
                 auto load_q = [&]() {
@@ -383,7 +403,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                 if (piece == 0) load_q();
                 auto ask = [&](int t) {
                     const int pos = t + lw * WR + lane;
-                    return pos < t1 && lane < WR ? __ldg(table + page_of(pos)) : 0;
+                    return pos < t1 && lane < WR ? tree_ask(table + page_of(pos)) : 0;
                 };
                 int id = ask(t0);
                 for (int j = 0; j < n; ++j) {
@@ -507,7 +527,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                 const int stage = (J0 + tile_of(X, i)) % NSV;
                 const uint32_t v_parity = v_par >> stage & 1;
                 v_par ^= 1u << stage;
-#pragma unroll
+#pragma unroll (MODE == 2 ? 2 : 1)
                 for (int h = 0; h < 2; ++h) {
                     wait_bar(bar_s + (X * 2 + h) * 8, C & 1);
                     __syncwarp();                                // the tensor-memory instructions want the whole warp
@@ -575,7 +595,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                         wait_bar(bar_o + (X * 2 + (h ^ 1)) * 8, (h ? C : C - 1) & 1);
                         __syncwarp();
                         tc::tc_fence_after();
-#pragma unroll
+#pragma unroll 1
                         for (int c0 = 0; c0 < DP; c0 += 32) {
                             uint32_t o[32];
                             tc::tmem_ld32(o_addr + c0, o);
@@ -638,7 +658,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                 s_ml[X * BM + row_l] = make_float2(m_run, l_run);
                 __syncwarp();
                 if (spread) {                                    // the columns that the other warp stores
-#pragma unroll
+#pragma unroll 1
                     for (int cc = 0; cc < COLS; cc += 32) {
                         uint32_t o[32];
                         tc::tmem_ld32(o_addr + (X ^ 1) * COLS + cc, o);
@@ -668,7 +688,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
             const long long at = tree_part_row(p, 2 * run_no + (b == run.b ? 0 : 1), kvh, row);
             if (write && !whole && (MODE != 1 || X == 0)) p.part_ml[at] = make_float2(m_all, l_all);
             T* dst = static_cast<T*>(p.out) + (((long long)b * p.tokens + tok) * p.q_heads + kvh * p.group + row - tok * p.group) * D;
-#pragma unroll
+#pragma unroll 1
             for (int cc = 0; cc < COLS; cc += 32) {
                 const int c0 = cc + (MODE == 1 ? X * COLS : 0);
                 uint32_t raw[32];
@@ -708,17 +728,6 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                     }
                 }
                 if (!write || c0 >= D) continue;
-                for (unsigned long long s = seen_bad; s; s &= s - 1ull) {
-                    const int t = prefix + __ffsll((long long)s) - 1;
-                    if (t < t0 || t >= t1) continue;             // (a drafted token of another piece)
-                    const T* vr = static_cast<const T*>(p.v) + tree_phys_row(p, table, t) * p.kv_heads * D + (long long)kvh * D + c0;
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        if (c0 + c >= D) continue;
-                        const float val = to_f32<T>(vr[c]);
-                        if ((__float_as_uint(val) & 0x7f800000u) == 0x7f800000u) o[c] += val;
-                    }
-                }
                 if (whole) {
 #pragma unroll
                     for (int c8 = 0; c8 < 4; ++c8) {
@@ -735,6 +744,22 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
 #pragma unroll
                     for (int c4 = 0; c4 < 8; ++c4)
                         if (c0 + c4 * 4 < D) acc[c4] = make_float4(o[c4 * 4], o[c4 * 4 + 1], o[c4 * 4 + 2], o[c4 * 4 + 3]);
+                }
+            }
+            // values that are not finite and that this row sees: added to what the thread has just stored
+            if (write) {
+                for (unsigned long long s = seen_bad; s; s &= s - 1ull) {
+                    const int t = prefix + __ffsll((long long)s) - 1;
+                    if (t < t0 || t >= t1) continue;             // (a drafted token of another piece)
+                    const T* vr = static_cast<const T*>(p.v) + tree_phys_row(p, table, t) * p.kv_heads * D + (long long)kvh * D;
+                    const int c1 = min(D, (MODE == 1 ? X * COLS : 0) + COLS);
+#pragma unroll 1
+                    for (int c = MODE == 1 ? X * COLS : 0; c < c1; ++c) {
+                        const float val = to_f32<T>(vr[c]);
+                        if ((__float_as_uint(val) & 0x7f800000u) != 0x7f800000u) continue;
+                        if (whole) dst[c] = from_f32<T>(to_f32<T>(dst[c]) + val);
+                        else p.part_acc[at * D + c] += val;
+                    }
                 }
             }
             __syncwarp();
