@@ -129,6 +129,12 @@ __device__ __forceinline__ unsigned long long tree_ask(const unsigned long long*
     asm volatile("ld.global.nc.b64 %0, [%1];" : "=l"(x) : "l"(at));
     return x;
 }
+// eight floats, a whole sector of memory, at once (a lane has a row, so a store of four fills half a sector
+// in each of 32 places: 16 bytes a lane took 4000 clocks a piece of 112 rows); 32-byte aligned
+__device__ __forceinline__ void tree_store8(float* at, const float* x) {
+    asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(at), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7]) : "memory");
+}
 // two lanes of packed fp32: d = a * b + c, d = a * b
 __device__ __forceinline__ void tree_fma2(float& d0, float& d1, float a0, float a1, float b, float c0, float c1) {
     asm("{\n\t.reg .b64 ra, rb, rc;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %4};\n\tmov.b64 rc, {%5, %6};\n\t"
@@ -740,10 +746,10 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                         *reinterpret_cast<uint4*>(dst + c0 + c8 * 8) = v;
                     }
                 } else {
-                    float4* acc = reinterpret_cast<float4*>(p.part_acc + at * D + c0);
+                    float* acc = p.part_acc + at * D + c0;       // (D is a multiple of 8)
 #pragma unroll
-                    for (int c4 = 0; c4 < 8; ++c4)
-                        if (c0 + c4 * 4 < D) acc[c4] = make_float4(o[c4 * 4], o[c4 * 4 + 1], o[c4 * 4 + 2], o[c4 * 4 + 3]);
+                    for (int c8 = 0; c8 < 32; c8 += 8)
+                        if (c0 + c8 < D) tree_store8(acc + c8, o + c8);
                 }
             }
             // values that are not finite and that this row sees: added to what the thread has just stored

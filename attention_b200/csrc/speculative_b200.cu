@@ -115,6 +115,9 @@ TreePlan tree_plan(int batch, int tokens, int q_heads, int kv_heads, long long c
     t.units = (long long)kv_heads * t.row_blocks;
     const long long cap_tiles = (long long)batch * ((cap_tokens + tile - 1) / tile);
     t.n_runs = tree_run_count(t.units, (long long)kSms * ctas_per_sm, cap_tiles);
+    // One sequence of a few tiles: a run that takes them all costs less than the merge (8 kv heads of D 128,
+    // 8 drafted tokens, one run / a run a tile: 2 tiles 8.7 / 11.4 us, 4 10.5 / 12.1, 6 12.3 / 12.9, 8 14.2 / 13.6).
+    if (batch == 1 && tile == kTreeTile && cap_tiles <= 6) t.n_runs = 1;
     return t;
 }
 TreePlan tree_plan_simt(int batch, int tokens, int q_heads, int kv_heads, long long cap_tokens) {
