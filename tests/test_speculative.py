@@ -343,6 +343,25 @@ def test_tree_work_split_over_runs(dtype, kernel, shape):
 
 
 @gpu
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [5, 128, 256, 257, 600, 768, 769, 1030])
+def test_tree_of_one_short_sequence(dtype, n, d):
+    """One run without a merge up to six tiles, a run a tile behind; infinite drafted values in both."""
+    t = 5
+    q, k, v, table, lens, mask, _ = case = tree_case([n], t, 6, 2, d, 16, dtype, seed=n)
+    check_tree(attn.gqa_tree_decode(*on_gpu(*case[:6])), case)
+    v = v.clone()
+    pos = n - t + 2
+    v[int(table[0, pos // 16]), pos % 16, 1, d - 1] = float("inf")
+    got = attn.gqa_tree_decode(*on_gpu(q, k, v, table, lens, mask)).cpu()
+    seen = ((mask[0] >> 2) & 1) == 1
+    want = torch.zeros(got.shape, dtype=torch.bool)
+    want[0, :, 3:, d - 1] = seen[:, None]
+    assert torch.equal(torch.isinf(got), want) and torch.isfinite(got[~want]).all()
+
+
+@gpu
 def test_tree_of_one_token_is_the_ordinary_decode_and_a_chain_needs_no_mask():
     case = tree_case([90, 400, 33], 1, 8, 2, 128, 16, torch.bfloat16, seed=2, masks=None)
     dq, dk, dv, dt, dl, _, _ = on_gpu(*case)
@@ -753,3 +772,25 @@ def test_front_doors_refuse_bad_tensors():
         attn.kv_copy_pages(k, v, lens, lens[:1])
     with pytest.raises(RuntimeError, match="int32"):
         attn.kv_copy_pages(k, v, lens.long(), lens.long())
+
+
+@gpu
+def test_moves_refuse_caches_that_share_memory():
+    """Both caches are moved by CTAs of their own: in shared memory one would read what the other has written."""
+    both = torch.zeros(2 * 6 * 16 * 2 * 64, dtype=torch.float16, device=DEV)
+    n = both.numel() // 2
+    shape = (6, 16, 2, 64)
+    k = both[:n].view(shape)
+    table = torch.zeros(2, 3, dtype=torch.int32, device=DEV)
+    src = torch.zeros(2, 4, dtype=torch.int32, device=DEV)
+    dst = torch.zeros(2, dtype=torch.int32, device=DEV)
+    rows = torch.zeros(2, 4, 2, 64, dtype=torch.float16, device=DEV)
+    cs = rope_table(16, 64).to(DEV)
+    for v in (k, both[64: 64 + n].view(shape)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            attn.kv_compact(k, v, table, src, dst)
+        with pytest.raises(RuntimeError, match="overlap"):
+            attn.kv_copy_pages(k, v, dst, dst)
+        with pytest.raises(RuntimeError, match="overlap"):
+            attn.qk_norm_rope_append(rows, rows, rows, None, None, cs, src, k, v, table)
+    attn.kv_copy_pages(k, both[n:].view(shape), dst, dst + 1)
