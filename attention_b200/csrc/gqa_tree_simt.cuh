@@ -16,6 +16,7 @@ namespace gqa_b200 {
 
 constexpr int kTreeSimtThreads = 128;
 constexpr int kTreeSimtKeys = 32;
+static_assert(kTreeSimtTile <= kTreeSimtThreads && kTreeSimtTile % kTreeSimtKeys == 0, "a thread finds a key of a tile");
 
 template <int RB, int DC> struct TreeSimtGeom {
     static constexpr int kLX = 2 * kTreeSimtThreads / RB;      // threads of a row pair
@@ -71,7 +72,8 @@ __global__ void __launch_bounds__(kTreeSimtThreads) gqa_tree_simt_kernel(const T
     float* s_k = s_q + RB * ST;                // [KN][ST]
     float* s_v = s_k + KN * ST;                // [KN][ST]
     float* s_p = s_v + KN * ST;                // [RB][PS]; a key that a row does not see holds -1
-    __shared__ long long s_off[RB > KN ? RB : KN];
+    __shared__ long long s_q_off[RB];
+    __shared__ long long s_off[kTreeSimtTile];   // of a whole tile's keys: its page ids are one trip to memory
     __shared__ long long s_scan[kTreeSimtThreads / 32 + 4];
 
     pdl_launch_dependents();
@@ -103,13 +105,18 @@ __global__ void __launch_bounds__(kTreeSimtThreads) gqa_tree_simt_kernel(const T
         const int32_t* table = p.table + (long long)b * p.max_pages;
 
         __syncthreads();                       // the piece before has left shared memory
+        auto find_keys = [&](int t) {          // pages of the keys t .. t + kTreeSimtTile - 1
+            if (tid < kTreeSimtTile)
+                s_off[tid] = t + tid < t1 ? tree_phys_row(p, table, t + tid) * p.kv_heads * D : -1;
+        };
         if (tid < RB) {
             const int row = row0 + tid, tok = row / p.group;
-            s_off[tid] = row < p.rows ? (((long long)b * p.tokens + tok) * p.q_heads + kvh * p.group + row - tok * p.group) * D
-                                      : -1;
+            s_q_off[tid] = row < p.rows ? (((long long)b * p.tokens + tok) * p.q_heads + kvh * p.group + row - tok * p.group) * D
+                                        : -1;
         }
+        find_keys(t0);
         __syncthreads();
-        tree_stage_rows<T, DC, RB>(s_q, ST, qp, s_off, D, vec);
+        tree_stage_rows<T, DC, RB>(s_q, ST, qp, s_q_off, D, vec);
 
         unsigned long long bits[2];
         bool live[2];
@@ -128,12 +135,16 @@ __global__ void __launch_bounds__(kTreeSimtThreads) gqa_tree_simt_kernel(const T
         }
 
         for (int t = t0; t < t1; t += KN) {
-            __syncthreads();                   // the keys before are done with (and s_off after the queries)
-            if (tid < KN)
-                s_off[tid] = t + tid < t1 ? tree_phys_row(p, table, t + tid) * p.kv_heads * D : -1;
-            __syncthreads();
-            tree_stage_rows<T, DC, KN>(s_k, ST, kp, s_off, D, vec);
-            tree_stage_rows<T, DC, KN>(s_v, ST, vp, s_off, D, vec);
+            const int in_tile = (t - t0) % kTreeSimtTile;
+            if (t > t0) {
+                __syncthreads();               // the keys before are done with
+                if (in_tile == 0) {
+                    find_keys(t);
+                    __syncthreads();
+                }
+            }
+            tree_stage_rows<T, DC, KN>(s_k, ST, kp, s_off + in_tile, D, vec);
+            tree_stage_rows<T, DC, KN>(s_v, ST, vp, s_off + in_tile, D, vec);
             __syncthreads();
             float s[2][LK];
 #pragma unroll
