@@ -8,7 +8,12 @@
 // the probabilities cross a warp, never the CTA, and the running maxima and sums stay in registers.
 // A warp reads a K element once for two rows (RB = 8) to eight (RB = 32): the shared-memory reads,
 // not the arithmetic, are what RB amortises, so few rows take the small block and many the large.
+// They are what bounds it: fp32, D 128, batch 16 of 1 to 4 k keys, 8 tokens 280 us (19 TFLOP/s), 32 tokens
+// 1010 us; 4 tokens at batch 64 786 us (1.7 TB/s).  A batch of four short sequences takes 28 us, most of
+// it trips to memory (lengths, page ids, keys) and the merge.
 #pragma once
+
+#include <type_traits>
 
 #include "gqa_tree_common.cuh"
 
@@ -29,30 +34,43 @@ template <int RB, int DC> struct TreeSimtGeom {
 };
 
 // N rows of D elements to shared memory as fp32, columns up to DC and rows whose offset is negative as
-// zeros.  All of a thread's loads are under way before the first is stored (one after the other, 16
-// round trips per 32 keys made most of the kernel's time).
-template <typename T, int DC, int N>
-__device__ __forceinline__ void tree_stage_rows(float* dst, int stride, const T* base, const long long* s_off, int D, bool vec) {
-    constexpr int V = 16 / (int)sizeof(T), C = DC / V;
-    if (vec) {
-        constexpr int PER = (N * C + kTreeSimtThreads - 1) / kTreeSimtThreads;
-        uint4 raw[PER];
+// zeros, in pieces of type U.  All of a thread's loads are under way before the first is stored (one after
+// the other, 16 round trips per 32 keys made most of the kernel's time).
+template <typename T, typename U, int DC, int N>
+__device__ __forceinline__ void tree_stage_pieces(float* dst, int stride, const T* base, const long long* s_off, int D) {
+    constexpr int V = (int)(sizeof(U) / sizeof(T)), C = DC / V;
+    constexpr int PER = (N * C + kTreeSimtThreads - 1) / kTreeSimtThreads;
+    U raw[PER];
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const int i = threadIdx.x + k * kTreeSimtThreads, r = i / C, c = (i - r * C) * V;
-            raw[k] = make_uint4(0u, 0u, 0u, 0u);
-            if (i < N * C && c < D && s_off[r] >= 0) raw[k] = __ldg(reinterpret_cast<const uint4*>(base + s_off[r] + c));
-        }
+    for (int k = 0; k < PER; ++k) {
+        const int i = threadIdx.x + k * kTreeSimtThreads, r = i / C, c = (i - r * C) * V;
+        raw[k] = U{};
+        if (i < N * C && c < D && s_off[r] >= 0) raw[k] = __ldg(reinterpret_cast<const U*>(base + s_off[r] + c));
+    }
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const int i = threadIdx.x + k * kTreeSimtThreads, r = i / C, c = (i - r * C) * V;
-            if (i >= N * C) continue;
-            const T* e = reinterpret_cast<const T*>(&raw[k]);
+    for (int k = 0; k < PER; ++k) {
+        const int i = threadIdx.x + k * kTreeSimtThreads, r = i / C, c = (i - r * C) * V;
+        if (i >= N * C) continue;
+        const T* e = reinterpret_cast<const T*>(&raw[k]);
+        if constexpr (V >= 4) {
 #pragma unroll
             for (int j = 0; j < V; j += 4)
                 *reinterpret_cast<float4*>(dst + r * stride + c + j) =
                     make_float4(to_f32<T>(e[j]), to_f32<T>(e[j + 1]), to_f32<T>(e[j + 2]), to_f32<T>(e[j + 3]));
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) dst[r * stride + c + j] = to_f32<T>(e[j]);
         }
+    }
+}
+// `piece` bytes divide every row and its address: 16, 4 (two 16-bit elements: 8 tokens on rows of 100
+// elements, batch 16, 305 us against 837 with one at a time), or one element.
+template <typename T, int DC, int N>
+__device__ __forceinline__ void tree_stage_rows(float* dst, int stride, const T* base, const long long* s_off, int D, int piece) {
+    if (piece == 16) {
+        tree_stage_pieces<T, uint4, DC, N>(dst, stride, base, s_off, D);
+    } else if (sizeof(T) == 2 && piece == 4) {
+        tree_stage_pieces<T, typename std::conditional<sizeof(T) == 2, unsigned, T>::type, DC, N>(dst, stride, base, s_off, D);
     } else {
 #pragma unroll 8
         for (int i = threadIdx.x; i < N * DC; i += kTreeSimtThreads) {
@@ -64,7 +82,7 @@ __device__ __forceinline__ void tree_stage_rows(float* dst, int stride, const T*
 }
 
 template <typename T, int RB, int DC>
-__global__ void __launch_bounds__(kTreeSimtThreads) gqa_tree_simt_kernel(const TreeParams p, const int vec) {
+__global__ void __launch_bounds__(kTreeSimtThreads) gqa_tree_simt_kernel(const TreeParams p, const int piece) {
     using G = TreeSimtGeom<RB, DC>;
     constexpr int KN = kTreeSimtKeys, LX = G::kLX, LK = G::kLK, NJ = G::kNJ, ST = G::kStride, PS = G::kPStride;
     extern __shared__ __align__(16) float s_tree[];
@@ -116,7 +134,7 @@ __global__ void __launch_bounds__(kTreeSimtThreads) gqa_tree_simt_kernel(const T
         }
         find_keys(t0);
         __syncthreads();
-        tree_stage_rows<T, DC, RB>(s_q, ST, qp, s_q_off, D, vec);
+        tree_stage_rows<T, DC, RB>(s_q, ST, qp, s_q_off, D, piece);
 
         unsigned long long bits[2];
         bool live[2];
@@ -143,8 +161,8 @@ __global__ void __launch_bounds__(kTreeSimtThreads) gqa_tree_simt_kernel(const T
                     __syncthreads();
                 }
             }
-            tree_stage_rows<T, DC, KN>(s_k, ST, kp, s_off + in_tile, D, vec);
-            tree_stage_rows<T, DC, KN>(s_v, ST, vp, s_off + in_tile, D, vec);
+            tree_stage_rows<T, DC, KN>(s_k, ST, kp, s_off + in_tile, D, piece);
+            tree_stage_rows<T, DC, KN>(s_v, ST, vp, s_off + in_tile, D, piece);
             __syncthreads();
             float s[2][LK];
 #pragma unroll

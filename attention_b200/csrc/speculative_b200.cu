@@ -167,18 +167,18 @@ inline long long cap_tokens_of(int max_pages, int block_size) {
 }
 
 template <typename T, int RB, int DC>
-cudaError_t launch_tree_simt(const TreeParams& p, const TreePlan& t, bool vec, cudaStream_t stream) {
+cudaError_t launch_tree_simt(const TreeParams& p, const TreePlan& t, int piece, cudaStream_t stream) {
     constexpr size_t smem = TreeSimtGeom<RB, DC>::kSmemBytes;
     auto kernel = gqa_tree_simt_kernel<T, RB, DC>;
     const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kernel), smem);
     if (e != cudaSuccess) return e;
-    return launch_pdl(kernel, dim3((unsigned)(t.n_runs * t.units)), kTreeSimtThreads, smem, stream, p, (int)vec);
+    return launch_pdl(kernel, dim3((unsigned)(t.n_runs * t.units)), kTreeSimtThreads, smem, stream, p, piece);
 }
 template <typename T, int RB>
-cudaError_t launch_tree_simt_dim(const TreeParams& p, const TreePlan& t, bool vec, cudaStream_t stream) {
-    if (p.head_dim <= 64) return launch_tree_simt<T, RB, 64>(p, t, vec, stream);
-    if (p.head_dim <= 128) return launch_tree_simt<T, RB, 128>(p, t, vec, stream);
-    return launch_tree_simt<T, RB, 256>(p, t, vec, stream);
+cudaError_t launch_tree_simt_dim(const TreeParams& p, const TreePlan& t, int piece, cudaStream_t stream) {
+    if (p.head_dim <= 64) return launch_tree_simt<T, RB, 64>(p, t, piece, stream);
+    if (p.head_dim <= 128) return launch_tree_simt<T, RB, 128>(p, t, piece, stream);
+    return launch_tree_simt<T, RB, 256>(p, t, piece, stream);
 }
 // cuTensorMapEncodeTiled, looked up through the runtime so that the library needs no link to the driver.
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -257,15 +257,15 @@ cudaError_t launch_tree_tc_dim(const TreeParams& p, const TreePlan& t, const Tre
     return launch_tree_tc<T, 256, 0, true>(p, t, *maps, stream);
 }
 template <typename T>
-cudaError_t launch_tree(const TreeParams& p, const TreePlan& t, bool tc, const TreeMaps* maps, bool vec, cudaStream_t stream) {
+cudaError_t launch_tree(const TreeParams& p, const TreePlan& t, bool tc, const TreeMaps* maps, int piece, cudaStream_t stream) {
     cudaError_t e = cudaErrorInvalidValue;
     if (tc) {
         if constexpr (sizeof(T) == 2) e = launch_tree_tc_dim<T>(p, t, maps, stream);
     } else {
         switch (t.row_block) {
-            case 8:  e = launch_tree_simt_dim<T, 8>(p, t, vec, stream); break;
-            case 16: e = launch_tree_simt_dim<T, 16>(p, t, vec, stream); break;
-            default: e = launch_tree_simt_dim<T, 32>(p, t, vec, stream); break;
+            case 8:  e = launch_tree_simt_dim<T, 8>(p, t, piece, stream); break;
+            case 16: e = launch_tree_simt_dim<T, 16>(p, t, piece, stream); break;
+            default: e = launch_tree_simt_dim<T, 32>(p, t, piece, stream); break;
         }
     }
     if (e != cudaSuccess || t.n_runs == 1) return e;
@@ -435,7 +435,10 @@ int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache
         if (block_size == 1 << s) p.bs_shift = s;
     p.cap_tokens = (int)cap;
     p.scale_log2 = scale * kLog2e;
-    const bool vec = head_dim * elem_size(dtype) % 16 == 0 && aligned16(q) && aligned16(k_cache) && aligned16(v_cache);
+    // bytes that rows are read by: what divides a row and the three addresses
+    const uintptr_t all = (uintptr_t)head_dim * elem_size(dtype) | reinterpret_cast<uintptr_t>(q) |
+                          reinterpret_cast<uintptr_t>(k_cache) | reinterpret_cast<uintptr_t>(v_cache);
+    const int piece = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : elem_size(dtype);
     TreeMaps maps{};
     const bool tma = tc && tree_tma_shape(p.group, head_dim, num_blocks, block_size, (long long)batch * tokens) &&
                      tree_maps(&maps, dtype == GQA_B200_BF16, p);
@@ -456,9 +459,9 @@ int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache
     p.row_blocks = plan.row_blocks;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (dtype) {
-        case GQA_B200_F32: return (int)launch_tree<float>(p, plan, tc, tma ? &maps : nullptr, vec, s);
-        case GQA_B200_F16: return (int)launch_tree<__half>(p, plan, tc, tma ? &maps : nullptr, vec, s);
-        default:           return (int)launch_tree<__nv_bfloat16>(p, plan, tc, tma ? &maps : nullptr, vec, s);
+        case GQA_B200_F32: return (int)launch_tree<float>(p, plan, tc, tma ? &maps : nullptr, piece, s);
+        case GQA_B200_F16: return (int)launch_tree<__half>(p, plan, tc, tma ? &maps : nullptr, piece, s);
+        default:           return (int)launch_tree<__nv_bfloat16>(p, plan, tc, tma ? &maps : nullptr, piece, s);
     }
 }
 

@@ -246,6 +246,15 @@ def test_tree_head_dims_and_pages(dtype, d, bs):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,hq", [(2, 4), (5, 4), (9, 6)])
+@pytest.mark.parametrize("d", [2, 50, 66, 100, 130, 202, 255])
+def test_tree_rows_that_are_not_whole_16_byte_pieces(dtype, t, hq, d):
+    case = tree_case([t + 1, 150, 64, 97], t, hq, 2, d, 16, dtype, seed=d)
+    check_tree(attn.gqa_tree_decode(*on_gpu(*case[:6])), case)
+
+
+@gpu
 @pytest.mark.parametrize("kernel", ["auto", "simt"])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_tree_lengths_and_draft_counts(dtype, kernel):
