@@ -134,6 +134,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_any_kernel(const
         const int e = lane + 32 * j;
         if (e >= D) continue;
         if (r.kind == 2) { dst[e] = from_f32<T>(x[j]); continue; }
+        if (!live) { dst[e] = from_f32<T>(0.f); continue; }   // (padding reads no angles: the table may be empty)
         float a = x[j] * rs * rope_weight<T>(p, r.kind, e);
         if (e < 2 * half) {
             const int o = p.interleaved ? e ^ 1 : (e < half ? e + half : e - half);
@@ -142,7 +143,7 @@ __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_any_kernel(const
             const float b = y[j] * rs * rope_weight<T>(p, r.kind, o);
             a = a * __ldg(cs + i) + (first ? -b : b) * __ldg(cs + half + i);
         }
-        dst[e] = from_f32<T>(live ? a : 0.f);
+        dst[e] = from_f32<T>(a);
     }
 }
 

@@ -176,6 +176,32 @@ def test_append_defaults_its_slots_to_the_positions_and_takes_one_token():
     assert int(torch.count_nonzero(vc.abs().sum((2, 3)))) == 3
 
 
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,rot,offset", [(128, 128, 0), (128, 64, 1), (5, 4, 0), (96, 12, 0)])
+def test_empty_angle_table_makes_every_token_padding(dtype, interleaved, d, rot, offset):
+    """No position lies inside a table of no rows: zeros come back, nothing is read from it and nothing written.
+    (`offset` 1, and sizes that are no multiples of 8, take the kernel for rows of any alignment.)"""
+    gen = torch.Generator().manual_seed(d)
+    b, t, hq, hkv = 2, 3, 4, 2
+    flat = torch.randn(b * t * hq * d + offset, generator=gen).to(dtype).to(DEV)
+    q = flat[offset:].view(b, t, hq, d)
+    k, v = torch.randn(2, b, t, hkv, d, generator=gen).to(dtype).to(DEV)
+    w = torch.ones(d, dtype=dtype, device=DEV)
+    cs = torch.empty(0, rot, device=DEV)
+    pos = torch.tensor([[0, -1, 5], [2**31 - 1, -2**31, 1]], dtype=torch.int32, device=DEV)
+    a, c = attn.qk_norm_rope(q, k, w, w, cs, pos, interleaved=interleaved)
+    assert torch.count_nonzero(a) == 0 and torch.count_nonzero(c) == 0
+    kc, vc = torch.randn(2, 4, 8, hkv, d, generator=gen).to(dtype).to(DEV)
+    keep = kc.clone(), vc.clone()
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=DEV)
+    slots = torch.arange(t, dtype=torch.int32, device=DEV).repeat(b, 1)
+    a = attn.qk_norm_rope_append(q, k, v, w, w, cs, pos, kc, vc, table, slots=slots, interleaved=interleaved)
+    assert torch.count_nonzero(a) == 0
+    assert torch.equal(kc, keep[0]) and torch.equal(vc, keep[1])
+
+
 # --------------------------------------------------------------------------- tree attention
 def tree_case(lengths, t, hq, hkv, d, bs, dtype, seed=0, drafts=None, masks="tree"):
     gen = torch.Generator().manual_seed(seed)
