@@ -60,8 +60,15 @@
 // of their own, and a chain's two halves share one body (MODE 2, bound by that body, has two):
 // 129 -> 117 us on the batch of 64 x 8 tokens, 45 -> 37 us on a ragged one of 32 x 16 tokens.
 //
-// Precision: scores and sums in fp32, P rounded to the element type (relative error half a step of
-// each probability, as in the other tensor-core kernels), O in fp32.
+// Precision: scores and sums in fp32, O in fp32, P rounded to the element type for the products.  In bf16
+// that is a relative error of half a step of each probability.  fp16 has that only down to 2^-14, and a key
+// that is 2^-25 of the row's reference would be nothing: many such keys below one whose value is small are
+// the result.  So fp16 probabilities are lifted by 2^kTreeLift, P = 2^(s - reference + lift), and the
+// reference follows the maximum more closely (kTreeSlack) to stay in range, P <= 2^15: half a step down to
+// 2^-25 of the largest, below that an absolute error of up to 2^-36 of it a key.  The lift is in P's sums as
+// well and cancels in their quotient; maxima that leave the chain are without it.  (Batch of 64 sequences of
+// 1 to 4 k keys, 16 tokens: no lift and a slack of 8, 128 us; 11 and 4, 130 to 135; 13 and 2, whose sums move
+// much more often, 147.  D 256, 64 tokens, batch 16: 130, 131 and 156.)
 #pragma once
 
 #include <cuda.h>
@@ -80,6 +87,10 @@ static __device__ int g_tree_tc_status;
 
 constexpr int kTreeBM = 128;            // rows of a query tile
 constexpr int kTreeTmemCols = 512;
+
+// log2 of what P is multiplied by, and how far a maximum may lie above its row's reference
+template <typename T> constexpr float kTreeLift = std::is_same<T, __half>::value ? 11.f : 0.f;
+template <typename T> constexpr float kTreeSlack = std::is_same<T, __half>::value ? 4.f : kRescaleSlack;
 
 template <int DP, int MODE> struct TreeTcGeom {
     static constexpr int kChains = MODE == 0 ? 1 : 2;
@@ -575,7 +586,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                         a1 = tc::max3(a1, sc[HN - 2], sc[HN - 1]);
                         mx = fmaxf(tc::max3(a0, a1, a2), a3) * p.scale_log2;
                     }
-                    const bool need = live && mx > m_run + kRescaleSlack;
+                    const bool need = live && mx > m_run + kTreeSlack<T>;
                     float alpha = 1.f;
                     if (need) {
                         const float mn = fmaxf(m_run, mx);
@@ -583,7 +594,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                         m_run = mn;
                         l_run *= alpha;
                     }
-                    const float nref = m_run == -INFINITY ? 0.f : -m_run;
+                    const float nref = m_run == -INFINITY ? 0.f : kTreeLift<T> - m_run;
 #pragma unroll
                     for (int c = 0; c < HN; c += 2) tc::fma2(sc[c], sc[c + 1], sc[c], sc[c + 1], p.scale_log2, nref);
 #pragma unroll

@@ -348,6 +348,37 @@ def test_tree_infinite_value_reaches_exactly_the_rows_that_see_it(dtype, kernel)
 
 @gpu
 @pytest.mark.parametrize("kernel", ["auto", "simt"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nats", [17.5, 20.0])
+@pytest.mark.parametrize("t,hq,d,bs", [(4, 4, 128, 16), (5, 20, 64, 16), (40, 8, 128, 16), (4, 4, 256, 16), (4, 4, 128, 24)])
+def test_tree_probabilities_far_below_a_dominating_key(dtype, kernel, nats, t, hq, d, bs):
+    """One key far above the others whose value is zero: the result is what the others weigh, e^-nats each.
+    In bf16 a rounded probability is off by h(t) of itself down to 2^-126.  In fp16 it is so down to the
+    smallest normal number, and below that off by at most half a step of 2^-24; the tensor-core kernel keeps
+    the row's largest at 2^11 or more, so relative to the largest that is 2^-25 / 2^11 = 2^-36 for a key, |v| 2^-36
+    in the result."""
+    lengths = [2500, 300, 1000]
+    q, k, v, table, lens, mask, _ = tree_case(lengths, t, hq, 2, d, bs, dtype, seed=t)
+    q[..., 0] = 8.0
+    k[..., 0] = 0.0
+    v = 256 * v.abs()
+    for b in range(len(lengths)):
+        page, line = int(table[b, 77 // bs]), 77 % bs
+        k[page, line] = 0.0
+        k[page, line, :, 0] = nats * math.sqrt(d) / 8.0
+        v[page, line] = 0.0
+    got = attn.gqa_tree_decode(*on_gpu(q, k, v, table, lens, mask), kernel=kernel).cpu().double()
+    want, mag = ref.tree_decode(q, k, v, table, lens, mask, None)
+    h = half_step(dtype)
+    size = float(q.double().norm(dim=-1).max()) * float(k.double().norm(dim=-1).max()) / math.sqrt(d)
+    fp32 = 2 * d * 2.0**-23 * size + 2.0**-20 + max(lengths) * 2.0**-23
+    p_round = 0.0 if dtype == torch.float32 else h
+    lowest = 2.0**-36 * max(lengths) * float(v.double().max()) if dtype == torch.float16 else 0.0
+    assert ((got - want).abs() <= h * want.abs() + (p_round + fp32) * mag + lowest + smallest(dtype)).all()
+
+
+@gpu
+@pytest.mark.parametrize("kernel", ["auto", "simt"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("shape", [(300, 3, 4, 2), (2, 7, 64, 64), (1, 64, 16, 2), (5, 20, 40, 8), (1, 1, 1, 1)])
 def test_tree_work_split_over_runs(dtype, kernel, shape):
