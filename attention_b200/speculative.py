@@ -57,17 +57,17 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
-def _check_out(out, like, name, inputs):
-    """A result buffer: contiguous, of `like`'s shape, and either `like` itself or apart from every input."""
+def _check_out(out, like, name, others):
+    """A result buffer: contiguous, of the shape of the input `like`, and either `like` itself or apart from it; apart
+    from the other inputs in any case (one of them may be the same tensor as `like`)."""
     if out is None:
         return torch.empty(like.shape, dtype=like.dtype, device=like.device)
     _check_cuda_contiguous(out, name)
     _check(out.shape == like.shape and out.dtype == like.dtype and out.device == like.device,
            f"{name} must have the shape, dtype and device of its input")
     same = out.data_ptr() == like.data_ptr() and like.is_contiguous()
-    for t in inputs:
-        if t is not None and not (same and t is like):
-            _check(not _overlap(out, t), f"{name} must not overlap an input other than the one it replaces")
+    _check((same or not _overlap(out, like)) and not any(t is not None and _overlap(out, t) for t in others),
+           f"{name} must not overlap an input other than the one it replaces")
     return out
 
 
@@ -149,7 +149,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, *, eps=1e-6, inte
     angles; the first ``R <= D`` elements are rotated, as pairs ``(i, i + R/2)`` or, ``interleaved``,
     ``(2i, 2i + 1)``.  ``positions`` int32 ``[B,T]`` (``[B]``); a token whose position is outside the
     table is padding and comes back as zeros.  Computed in fp32, rounded once.  Returns contiguous
-    ``(q_out, k_out)``; a given ``q_out`` / ``k_out`` may be ``q`` / ``k`` itself.  No autograd support.
+    ``(q_out, k_out)``; a given ``q_out`` / ``k_out`` may be ``q`` / ``k`` itself and must be apart from the
+    other inputs.  No autograd support.
     """
     lib = _lib()
     eps = float(eps)
@@ -164,9 +165,9 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos_sin, positions, *, eps=1e-6, inte
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     else:
-        both = (q, k, q_weight, k_weight, cos_sin, positions)
-        q_out = _check_out(q_out, q, "q_out", both)
-        k_out = _check_out(k_out, k, "k_out", both)
+        rest = (q_weight, k_weight, cos_sin, positions)
+        q_out = _check_out(q_out, q, "q_out", (k, *rest))
+        k_out = _check_out(k_out, k, "k_out", (q, *rest))
         _check(not _overlap(q_out, k_out), "q_out and k_out must not overlap")
     four = len(qs) == 4
     tokens = qs[1] if four else 1
@@ -246,7 +247,7 @@ def qk_norm_rope_append(q, k, v, q_weight, k_weight, cos_sin, positions, k_cache
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
-        out = _check_out(out, q, "out", (q, k, v, q_weight, k_weight, cos_sin, positions, slots, k_cache, v_cache,
+        out = _check_out(out, q, "out", (k, v, q_weight, k_weight, cos_sin, positions, slots, k_cache, v_cache,
                                          block_table))
     four = len(qs) == 4
     tokens = qs[1] if four else 1

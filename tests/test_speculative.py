@@ -860,3 +860,21 @@ def test_moves_refuse_caches_that_share_memory():
         with pytest.raises(RuntimeError, match="overlap"):
             attn.qk_norm_rope_append(rows, rows, rows, None, None, cs, src, k, v, table)
     attn.kv_copy_pages(k, both[n:].view(shape), dst, dst + 1)
+
+
+@gpu
+def test_norm_rope_in_place_refuses_a_tensor_that_is_queries_and_keys():
+    """The heads of both are worked on side by side: rows that are still to be read would be overwritten."""
+    x = torch.zeros(2, 3, 4, 64, dtype=torch.float16, device=DEV)
+    cs = rope_table(16, 64).to(DEV)
+    pos = torch.zeros(2, 3, dtype=torch.int32, device=DEV)
+    kc, vc = torch.zeros(2, 4, 16, 4, 64, dtype=torch.float16, device=DEV)
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=DEV)
+    for change in (dict(q_out=x), dict(k_out=x)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            attn.qk_norm_rope(x, x, None, None, cs, pos, **change)
+    for k, v in ((x, x.clone()), (x.clone(), x)):
+        with pytest.raises(RuntimeError, match="overlap"):
+            attn.qk_norm_rope_append(x, k, v, None, None, cs, pos, kc, vc, table, out=x)
+    a, b = attn.qk_norm_rope(x, x, None, None, cs, pos)         # as two inputs it is as good as any other
+    assert a.data_ptr() != b.data_ptr()
