@@ -450,6 +450,7 @@ const char* gqa_b200_strerror(int code) {
         case GQA_B200_ERR_ROTATION:
             return "rot_dim must be even and in [0, head_dim], max_position in [0, 2^31)";
         case GQA_B200_ERR_COMPACT_ROWS: return "kv_compact moves at most 1024 rows per sequence";
+        case GQA_B200_ERR_OVERLAP: return "memory that is written must not overlap an input";
         case MLA_B200_ERR_SHAPE: return "MLA: a width, head count, tq or nk is not positive";
         case MLA_B200_ERR_LATENT_DIM: return "MLA: supported latent width dc is [1, 512]";
         default: break;

@@ -33,6 +33,24 @@ inline bool known_dtype(int dtype) {
     return dtype == GQA_B200_F32 || dtype == GQA_B200_F16 || dtype == GQA_B200_BF16;
 }
 
+// A range of addresses, [lo, hi).
+struct Span {
+    uintptr_t lo, hi;
+    bool meets(const Span& o) const { return lo < o.hi && o.lo < hi; }
+};
+inline Span span_of(const void* p, size_t bytes) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    return Span{a, a + bytes};
+}
+// ... of `heads` rows of `dim` elements for each of batch * tokens tokens, strides in elements
+Span span_of_rows(const void* p, int batch, int tokens, int heads, int dim, const int64_t* strides, int size) {
+    int64_t lo = 0, hi = dim;
+    const int n[3] = {batch, tokens, heads};
+    for (int i = 0; i < 3; ++i) (strides[i] < 0 ? lo : hi) += (n[i] - 1) * strides[i];
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    return Span{a + lo * size, a + hi * size};
+}
+
 std::mutex g_mutex;                          // guards the per-device caches of this file
 
 bool pdl_on() {
@@ -360,6 +378,14 @@ int gqa_b200_qk_norm_rope(const void* q, const void* k, const void* v, const voi
         if (max_pages <= 0) return GQA_B200_ERR_MAX_PAGES;
         if (num_blocks > kIntMax) return GQA_B200_ERR_INT32_RANGE;
         if (!v || !v_cache || !block_table || !slots) return GQA_B200_ERR_NULL_POINTER;
+        // a row that is still to be read must not be another token's place in the cache
+        const size_t size = elem_size(dtype), cache = (size_t)num_blocks * block_size * kv_heads * head_dim * size;
+        const Span caches[2] = {span_of(k_cache, cache), span_of(v_cache, cache)};
+        for (const Span& c : caches)
+            if (c.meets(span_of_rows(q, batch, tokens, q_heads, head_dim, strides, (int)size)) ||
+                c.meets(span_of_rows(k, batch, tokens, kv_heads, head_dim, strides + 3, (int)size)) ||
+                c.meets(span_of_rows(v, batch, tokens, kv_heads, head_dim, strides + 6, (int)size)))
+                return GQA_B200_ERR_OVERLAP;
     } else if (!k_out) {
         return GQA_B200_ERR_NULL_POINTER;
     }

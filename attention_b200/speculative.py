@@ -227,8 +227,8 @@ def qk_norm_rope_append(q, k, v, q_weight, k_weight, cos_sin, positions, k_cache
     The row of token ``t`` of sequence ``b`` is written to position ``slots[b,t]`` (int32, default
     ``positions``) of its pages: page ``block_table[b, slot // block_size]``, row ``slot % block_size``.
     ``positions`` are the rotation's; the tokens of a tree share positions and differ in slots.  Nothing
-    is written for padding (a position outside ``cos_sin``) or for a slot or page out of range; the
-    caller owns distinct destinations.  Returns the rotated queries, shaped as ``q`` and contiguous;
+    is written for padding (a position outside ``cos_sin``) or for a slot or page out of range; ``q``, ``k``
+    and ``v`` must not overlap the caches, and the caller owns distinct destinations.  Returns the rotated queries, shaped as ``q`` and contiguous;
     ``out`` may be ``q`` itself.  No autograd support.
     """
     lib = _lib()

@@ -67,6 +67,7 @@ extern "C" {
 #define GQA_B200_ERR_TREE_TOKENS (-15) /* drafted tokens per sequence must be in [1, 64] */
 #define GQA_B200_ERR_ROTATION (-16)   /* rot_dim must be even, in [0, head_dim]; max_position in [0, 2^31) */
 #define GQA_B200_ERR_COMPACT_ROWS (-17) /* at most 1024 rows per sequence in one kv_compact */
+#define GQA_B200_ERR_OVERLAP (-18)    /* memory that is written must not overlap an input */
 
 /* Workspace header: the first int32 words of the workspace, readable by the
  * host after a stream synchronise when debugging.
@@ -285,8 +286,9 @@ GQA_B200_API int gqa_b200_kv_append(const void* key, const void* value, void* k_
  * k_cache null: dense form, keys go to k_out (as q_out; v and the cache arguments
  * are ignored).  Otherwise keys and values of token t of sequence b go to position
  * slots[b, t] of the sequence's pages (layout and block_table as above), nothing is
- * written for padding, slots outside the table or pages outside the pool.  The
- * caller owns distinct destinations. */
+ * written for padding, slots outside the table or pages outside the pool.  q, k and v
+ * must lie outside the caches (GQA_B200_ERR_OVERLAP); the caller owns distinct
+ * destinations. */
 GQA_B200_API int gqa_b200_qk_norm_rope(const void* q, const void* k, const void* v,
                                        const void* q_weight, const void* k_weight,
                                        const float* cos_sin, const int32_t* positions, void* q_out,

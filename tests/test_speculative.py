@@ -768,6 +768,54 @@ def test_c_entry_points_refuse_bad_arguments():
     assert copy(n=0) == 0 and copy(blocks=2**31) == -13
 
 
+def test_append_refuses_rows_that_lie_in_the_caches():
+    """Another token's write could reach a row before it is read.  (Addresses only: nothing is launched.)"""
+    lib = _cabi.load()
+    b, t, hq, hkv, d, blocks, bs = 2, 3, 4, 2, 64, 5, 16
+    cache = blocks * bs * hkv * d * 2
+    kc, vc, rest = 1 << 20, (1 << 20) + 2 * cache, 1 << 30
+    q_bytes, kv_bytes = b * t * hq * d * 2, b * t * hkv * d * 2
+
+    def call(q=rest, k=rest + (1 << 20), v=rest + (2 << 20), st=None):
+        st = st or [t * hq * d, hq * d, d] + [t * hkv * d, hkv * d, d] * 2
+        out, meta = 1 << 40, 1 << 41
+        return lib.gqa_b200_qk_norm_rope(q, k, v, None, None, meta, meta, out, None, kc, vc, meta, meta, 2, 2, b, t, hq, hkv,
+                                         d, d, 10, (ctypes.c_int64 * 9)(*st), 1e-6, 0, blocks, bs, 4, None)
+
+    for base in (kc, vc):
+        assert call(q=base - q_bytes + 2) == -18 and call(q=base + cache - 2) == -18
+        assert call(k=base) == -18 and call(k=base + cache - 128) == -18
+        assert call(v=base - kv_bytes + 2) == -18 and call(v=base + cache // 2) == -18
+    # rows before the address, by a negative stride; a token's rows far behind it
+    assert call(k=kc + cache, st=[t * hq * d, hq * d, d, -t * hkv * d, hkv * d, d, t * hkv * d, hkv * d, d]) == -18
+    assert call(v=kc - 4 * kv_bytes, st=[t * hq * d, hq * d, d, t * hkv * d, hkv * d, d, 2 * kv_bytes, hkv * d, d]) == -18
+    assert "overlap" in _cabi.strerror(-18)
+
+
+@gpu
+def test_append_takes_rows_that_border_on_the_caches():
+    """Queries, keys, values and both caches side by side in one allocation, and a key among the cache's rows refused."""
+    b, t, hkv, d, pages, bs = 2, 3, 2, 64, 4, 16
+    rows, cache = b * t * hkv * d, pages * bs * hkv * d
+    gen = torch.Generator().manual_seed(0)
+    flat = torch.randn(3 * rows + 2 * cache, generator=gen).half().to(DEV)
+    q, kc, k, vc, v = (x.view(-1, bs, hkv, d) if x.numel() == cache else x.view(b, t, hkv, d)
+                       for x in flat.split([rows, cache, rows, cache, rows]))
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=DEV)
+    pos = torch.tensor([[0, 17, 31], [5, 6, 7]], dtype=torch.int32, device=DEV)
+    cs = rope_table(40, d).to(DEV)
+    want_k, want_v = kc.cpu(), vc.cpu()
+    with pytest.raises(RuntimeError, match="overlap"):
+        attn.qk_norm_rope_append(q, kc.view(-1)[:rows].view(b, t, hkv, d), v, None, None, cs, pos, kc, vc, table)
+    assert torch.equal(kc.cpu(), want_k) and torch.equal(vc.cpu(), want_v)
+    keys = attn.qk_norm_rope(q, k, None, None, cs, pos)[1].cpu()
+    attn.qk_norm_rope_append(q, k, v, None, None, cs, pos, kc, vc, table)
+    live = torch.ones(b, t, dtype=torch.bool)
+    ref.write_rows(want_k, keys, table.cpu(), pos.cpu(), live)
+    ref.write_rows(want_v, v.cpu(), table.cpu(), pos.cpu(), live)
+    assert torch.equal(kc.cpu(), want_k) and torch.equal(vc.cpu(), want_v)
+
+
 def test_front_doors_refuse_cpu_tensors():
     q = torch.zeros(2, 3, 4, 64)
     cache = torch.zeros(4, 16, 2, 64)
