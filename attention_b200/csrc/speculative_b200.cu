@@ -474,9 +474,20 @@ int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache
     if (plan.n_runs * plan.units > kIntMax || cap_tiles / plan.n_runs >= kIntMax / 2) return GQA_B200_ERR_INT32_RANGE;
     const TreeScratch lay = tree_scratch(plan, tokens, q_heads, head_dim);
     // (the published size, whichever kernel runs)
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) ||
-        workspace_bytes < gqa_b200_tree_workspace_bytes(batch, tokens, q_heads, kv_heads, head_dim, block_size, max_pages))
-        return GQA_B200_ERR_WORKSPACE;
+    const size_t need = gqa_b200_tree_workspace_bytes(batch, tokens, q_heads, kv_heads, head_dim, block_size, max_pages);
+    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255u) || workspace_bytes < need) return GQA_B200_ERR_WORKSPACE;
+    // scratch and result are written while the inputs are read, and scratch is read after the first results are written
+    const size_t size = elem_size(dtype), rows = (size_t)batch * tokens * q_heads * head_dim * size;
+    const size_t cache = (size_t)num_blocks * block_size * kv_heads * head_dim * size;
+    const Span scratch = span_of(workspace, need), result = span_of(out, rows);
+    const Span inputs[7] = {span_of(q, rows), span_of(k_cache, cache), span_of(v_cache, cache),
+                            span_of(block_table, (size_t)batch * max_pages * sizeof(int32_t)),
+                            span_of(context_lens, batch * sizeof(int32_t)),
+                            span_of(draft_lens, draft_lens ? batch * sizeof(int32_t) : 0),
+                            span_of(tree_mask, tree_mask ? (size_t)batch * tokens * sizeof(int64_t) : 0)};
+    if (scratch.meets(result)) return GQA_B200_ERR_OVERLAP;
+    for (const Span& x : inputs)
+        if (scratch.meets(x) || result.meets(x)) return GQA_B200_ERR_OVERLAP;
     char* ws = static_cast<char*>(workspace);
     p.info = reinterpret_cast<int4*>(ws + lay.info);
     p.part_ml = reinterpret_cast<float2*>(ws + lay.ml);

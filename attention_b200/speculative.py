@@ -346,7 +346,7 @@ def gqa_tree_decode(q, k_cache, v_cache, block_table, context_lens, tree_mask=No
     ``tree_mask[b,i]`` (int64 ``[B,T]``, default the chain ``0 .. i``).  Rows that see nothing and rows
     from ``draft_lens[b]`` on come back as zeros; keys and values that a row does not see may hold
     anything.  ``workspace`` (uint8, at least ``tree_workspace_bytes(...)``, 256-byte aligned, contents
-    irrelevant) is taken from the allocator for each call by default, so calls on different streams and
+    irrelevant, apart from ``out`` and the inputs) is taken from the allocator for each call by default, so calls on different streams and
     captured graphs share nothing.  ``kernel``: ``"auto" | "simt" | "tcgen05"``.  No autograd support.
     """
     lib = _lib()

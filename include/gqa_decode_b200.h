@@ -314,7 +314,8 @@ GQA_B200_API size_t gqa_b200_tree_workspace_bytes(int batch, int tokens, int q_h
  * before the drafted ones and drafted token j iff bit j of tree_mask[b, i] is set
  * (int64 [batch, tokens]; null: bits 0 .. i, a chain).  A row that sees nothing, and
  * rows from draft_lens[b] on, are zeros.  Keys and values that a row does not see
- * may hold anything, infinities and NaN included.  kernel: GQA_B200_KERNEL_AUTO,
+ * may hold anything, infinities and NaN included.  `out` and the workspace must not
+ * overlap an input or one another (GQA_B200_ERR_OVERLAP).  kernel: GQA_B200_KERNEL_AUTO,
  * _SIMT, or _TCGEN05 (fp16/bf16, rows of head_dim elements a multiple of 16 bytes,
  * 16-byte aligned tensors, num_blocks * block_size < 2^32; what AUTO picks for those). */
 GQA_B200_API int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache,

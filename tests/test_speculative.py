@@ -816,6 +816,48 @@ def test_append_takes_rows_that_border_on_the_caches():
     assert torch.equal(kc.cpu(), want_k) and torch.equal(vc.cpu(), want_v)
 
 
+def test_tree_refuses_a_workspace_that_meets_result_or_inputs():
+    """(Addresses only: nothing is launched.)"""
+    lib = _cabi.load()
+    b, t, hq, hkv, d, blocks, bs, pages = 3, 4, 8, 2, 64, 40, 16, 12
+    need = lib.gqa_b200_tree_workspace_bytes(b, t, hq, hkv, d, bs, pages)
+    assert need > 4096
+    size = dict(q=b * t * hq * d * 2, k=blocks * bs * hkv * d * 2, v=blocks * bs * hkv * d * 2, table=b * pages * 4, lens=b * 4,
+                drafts=b * 4, mask=b * t * 8, out=b * t * hq * d * 2)
+    at = {name: (i + 1) << 30 for i, name in enumerate(size)}
+    names = ("q", "k", "v", "table", "lens", "drafts", "mask", "out")
+
+    def call(ws, **change):
+        a = {**at, **change}
+        return lib.gqa_b200_tree_decode(*(a[n] for n in names), 2, b, t, hq, hkv, d, blocks, bs, pages, 0.1, 0, ws, need, None)
+
+    for name in names:
+        ws = (at[name] + size[name] - 1) // 256 * 256           # begins in the buffer's last bytes
+        assert call(ws) == -18, name
+        assert call(1 << 40, **{name: (1 << 40) + need - 1}) == -18, name
+        assert call(1 << 40, **{name: (1 << 40) - size[name] + 1}) == -18, name
+    for name in names[:-1]:
+        assert call(1 << 40, out=at[name] + size[name] - 1) == -18, name
+
+
+@gpu
+def test_tree_workspace_may_border_on_result_and_inputs():
+    case = tree_case([100, 17, 260], 4, 8, 2, 64, 16, torch.float16, seed=9)
+    dq, dk, dv, dt, dl, dm, _ = on_gpu(*case)
+    need = attn.tree_workspace_bytes(3, 4, 8, 2, 64, 16, dt.shape[1])
+    flat = torch.empty(need + 2 * dq.nbytes, dtype=torch.uint8, device=DEV)
+    assert dq.nbytes % 256 == 0
+    q, ws, out = flat.split([dq.nbytes, need, dq.nbytes])
+    q, out = q.view(dq.dtype).view(dq.shape), out.view(dq.dtype).view(dq.shape)
+    q.copy_(dq)
+    with pytest.raises(RuntimeError, match="overlap"):
+        attn.gqa_tree_decode(q, dk, dv, dt, dl, dm, workspace=flat[: need])
+    with pytest.raises(RuntimeError, match="overlap"):
+        attn.gqa_tree_decode(q, dk, dv, dt, dl, dm, out=out, workspace=flat[2 * dq.nbytes:])
+    check_tree(attn.gqa_tree_decode(q, dk, dv, dt, dl, dm, out=out, workspace=ws), case)
+    assert torch.equal(q, dq)
+
+
 def test_front_doors_refuse_cpu_tensors():
     q = torch.zeros(2, 3, 4, 64)
     cache = torch.zeros(4, 16, 2, 64)
