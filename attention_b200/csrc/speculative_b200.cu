@@ -297,25 +297,25 @@ cudaError_t launch_tree(const TreeParams& p, const TreePlan& t, bool tc, const T
 }
 
 // ---------------------------------------------------------------------------
-// norm and rotation
+// norm and rotation (these return a status of the C interface)
 // ---------------------------------------------------------------------------
 template <typename T, int L, int HB>
-cudaError_t launch_rope_vec(const RopeParams& p, cudaStream_t stream) {
+int launch_rope_vec(const RopeParams& p, cudaStream_t stream) {
     RopeBlocks blocks;
     blocks.q = (unsigned)((p.q_heads + HB - 1) / HB);
     blocks.k = (unsigned)((p.kv_heads + HB - 1) / HB);
     blocks.all = blocks.q + blocks.k * (p.append ? 2 : 1);
     const long long units = p.n_tokens * blocks.all, groups = kRopeThreads / L;
-    if (units > kIntMax) return cudaErrorInvalidValue;
+    if (units > kIntMax) return GQA_B200_ERR_INT32_RANGE;
     auto kernel = p.interleaved ? qk_norm_rope_vec_kernel<T, L, HB, true> : qk_norm_rope_vec_kernel<T, L, HB, false>;
     kernel<<<(unsigned)((units + groups - 1) / groups), kRopeThreads, 0, stream>>>(p, blocks, (unsigned)units);
-    return cudaGetLastError();
+    return (int)cudaGetLastError();
 }
 template <typename T, int L>
-cudaError_t launch_rope_heads(const RopeParams& p, int heads, cudaStream_t stream) {
+int launch_rope_heads(const RopeParams& p, int heads, cudaStream_t stream) {
     // Several heads per group once that still gives every SM its fill of threads: the 32 bytes of angles
     // that a lane reads from the first-level cache then serve as many 16-byte pieces of rows.
-        // (Dense 16384 tokens x 72 heads of 128 bf16: 854 us with a warp per row, 154 with two heads per group,
+    // (Dense 16384 tokens x 72 heads of 128 bf16: 854 us with a warp per row, 154 with two heads per group,
     // 116 with four, 151 with eight, whose registers leave fewer warps.)
     constexpr int HB = 4;
     return p.n_tokens * heads * L >= (long long)HB * kSms * 1024 ? launch_rope_vec<T, L, HB>(p, stream)
@@ -335,7 +335,7 @@ bool rope_vec_ok(const RopeParams& p, int size) {
 }
 
 template <typename T>
-cudaError_t launch_rope(const RopeParams& p, cudaStream_t stream) {
+int launch_rope(const RopeParams& p, cudaStream_t stream) {
     const int heads = p.q_heads + p.kv_heads * (p.append ? 2 : 1);
     if (rope_vec_ok(p, (int)sizeof(T))) {
         if (p.head_dim <= 64) return launch_rope_heads<T, 8>(p, heads, stream);
@@ -344,9 +344,9 @@ cudaError_t launch_rope(const RopeParams& p, cudaStream_t stream) {
     }
     const long long rows = p.n_tokens * heads;
     const long long grid = (rows + kRopeWarps - 1) / kRopeWarps;
-    if (grid > kIntMax) return cudaErrorInvalidValue;
+    if (grid > kIntMax) return GQA_B200_ERR_INT32_RANGE;
     qk_norm_rope_any_kernel<T><<<(unsigned)grid, kRopeWarps * 32, 0, stream>>>(p);
-    return cudaGetLastError();
+    return (int)cudaGetLastError();
 }
 
 }  // namespace
@@ -405,9 +405,9 @@ int gqa_b200_qk_norm_rope(const void* q, const void* k, const void* v, const voi
     p.eps = eps;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     switch (dtype) {
-        case GQA_B200_F32: return (int)launch_rope<float>(p, s);
-        case GQA_B200_F16: return (int)launch_rope<__half>(p, s);
-        default:           return (int)launch_rope<__nv_bfloat16>(p, s);
+        case GQA_B200_F32: return launch_rope<float>(p, s);
+        case GQA_B200_F16: return launch_rope<__half>(p, s);
+        default:           return launch_rope<__nv_bfloat16>(p, s);
     }
 }
 

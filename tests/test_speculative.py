@@ -858,6 +858,19 @@ def test_tree_workspace_may_border_on_result_and_inputs():
     assert torch.equal(q, dq)
 
 
+def test_norm_rope_of_too_many_rows_has_a_status_of_its_own():
+    """More groups of rows than a launch can number: the same status as the other sizes that exceed one."""
+    lib = _cabi.load()
+
+    def call(d, heads, batch=2**31 - 1, tokens=2):
+        strides = (ctypes.c_int64 * 9)(*([0] * 9))
+        return lib.gqa_b200_qk_norm_rope(16, 16, None, None, None, 16, 16, 16, 16, None, None, None, None, 2, 2, batch, tokens,
+                                         heads, heads, d, d // 2 * 2, 10, strides, 1e-6, 0, 0, 0, 0, None)
+
+    assert call(128, 1) == -13 and call(64, 4) == -13 and call(256, 8) == -13       # rows of whole chunks
+    assert call(5, 4) == -13                                                        # the kernel for any row
+
+
 def test_front_doors_refuse_cpu_tensors():
     q = torch.zeros(2, 3, 4, 64)
     cache = torch.zeros(4, 16, 2, 64)
