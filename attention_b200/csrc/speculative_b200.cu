@@ -25,6 +25,7 @@ namespace {
 constexpr int kSms = 148;                    // the cut of the work is for a B200, whatever runs it
 constexpr int kTreeSimtCtasPerSm = 3;
 constexpr long long kIntMax = 0x7fffffffll;
+constexpr long long kTreeMaxRows = 1 << 20;  // tokens x q_heads of a sequence: row numbers are int32
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline int elem_size(int dtype) { return dtype == GQA_B200_F32 ? 4 : 2; }
@@ -414,7 +415,7 @@ int gqa_b200_qk_norm_rope(const void* q, const void* k, const void* v, const voi
 size_t gqa_b200_tree_workspace_bytes(int batch, int tokens, int q_heads, int kv_heads, int head_dim, int block_size,
                                      int max_pages) {
     if (batch <= 0 || tokens <= 0 || tokens > kTreeMaxTokens || q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads ||
-        head_dim <= 0 || head_dim > 256 || block_size <= 0 || max_pages <= 0)
+        head_dim <= 0 || head_dim > 256 || block_size <= 0 || max_pages <= 0 || (long long)tokens * q_heads > kTreeMaxRows)
         return 0;
     const long long cap = cap_tokens_of(max_pages, block_size);
     // any of the kernels may run: which one depends on types, addresses and the size of the pool
@@ -439,7 +440,7 @@ int gqa_b200_tree_decode(const void* q, const void* k_cache, const void* v_cache
     if (num_blocks <= 0 || block_size <= 0) return GQA_B200_ERR_CACHE_SHAPE;
     if (max_pages <= 0) return GQA_B200_ERR_MAX_PAGES;
     if (!(std::isfinite(scale) && scale > 0.f)) return GQA_B200_ERR_SCALE;
-    if (num_blocks > kIntMax || (long long)tokens * q_heads > (1 << 20)) return GQA_B200_ERR_INT32_RANGE;
+    if (num_blocks > kIntMax || (long long)tokens * q_heads > kTreeMaxRows) return GQA_B200_ERR_INT32_RANGE;
     if (kernel != GQA_B200_KERNEL_AUTO && kernel != GQA_B200_KERNEL_SIMT && kernel != GQA_B200_KERNEL_TCGEN05)
         return GQA_B200_ERR_KERNEL;
     if (batch == 0) return GQA_B200_OK;

@@ -340,7 +340,7 @@ def gqa_tree_decode(q, k_cache, v_cache, block_table, context_lens, tree_mask=No
                     out=None, workspace=None, kernel="auto"):
     """Paged GQA attention of up to 64 drafted tokens per sequence.
 
-    ``q [B,T,Hq,D]``, caches, ``block_table`` and ``context_lens`` as for ``gqa_decode``; the lengths
+    ``q [B,T,Hq,D]`` (``T * Hq <= 2**20``), caches, ``block_table`` and ``context_lens`` as for ``gqa_decode``; the lengths
     count the drafted tokens, which are the last ``draft_lens[b]`` (int32 ``[B]``, default ``T``) keys of
     a sequence.  Row ``i`` sees every earlier key and drafted token ``j`` iff bit ``j`` of
     ``tree_mask[b,i]`` (int64 ``[B,T]``, default the chain ``0 .. i``).  Rows that see nothing and rows

@@ -301,8 +301,9 @@ GQA_B200_API int gqa_b200_qk_norm_rope(const void* q, const void* k, const void*
                                        void* stream);
 
 /* Bytes of scratch gqa_b200_tree_decode needs for this static shape, 256-byte
- * aligned.  Its contents need not be initialised and nothing carries over between
- * calls; calls that may overlap on the device need buffers of their own. */
+ * aligned; 0 for a shape that gqa_b200_tree_decode refuses (more than 2^20 query rows
+ * tokens * q_heads among them).  Its contents need not be initialised and nothing carries
+ * over between calls; calls that may overlap on the device need buffers of their own. */
 GQA_B200_API size_t gqa_b200_tree_workspace_bytes(int batch, int tokens, int q_heads, int kv_heads,
                                                   int head_dim, int block_size, int max_pages);
 

@@ -871,6 +871,14 @@ def test_norm_rope_of_too_many_rows_has_a_status_of_its_own():
     assert call(5, 4) == -13                                                        # the kernel for any row
 
 
+def test_tree_workspace_of_too_many_rows_is_nothing():
+    """tokens x q_heads beyond 2^20 is refused by the call: no scratch is asked for, and no int32 overflows on the way."""
+    ws = _cabi.load().gqa_b200_tree_workspace_bytes
+    assert ws(1, 64, 2**14, 2**14, 64, 16, 64) > 0
+    for tokens, q_heads, kv_heads in [(64, 2**14 + 1, 1), (64, 2**30, 1), (33, 2**26, 1), (1, 2**20 + 1, 1), (64, 2**30, 2**30)]:
+        assert ws(1, tokens, q_heads, kv_heads, 64, 16, 64) == 0
+
+
 def test_front_doors_refuse_cpu_tensors():
     q = torch.zeros(2, 3, 4, 64)
     cache = torch.zeros(4, 16, 2, 64)
