@@ -274,6 +274,14 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
         }
     };
 
+    // The loaders' wait: their lanes work together (shuffles, __syncwarp), so all of them leave off or none.  (The MMA
+    // warps' products hang on one lane, and the softmax warps go through their hand-offs either way.)
+    auto wait_together = [&](uint32_t bar, uint32_t parity) {
+        if (__all_sync(0xffffffffu, tc::mbar_test(bar, parity))) return;
+        wait_bar(bar, parity);
+        alive = __all_sync(0xffffffffu, alive);
+    };
+
     // 16-byte chunk of a row that this lane copies, and the rows a pass of the warp covers
     constexpr int CPRW = DP / 8, RPI = 32 / CPRW;
     const int ld_c = lane % CPRW, ld_row0 = lane / CPRW;
@@ -378,7 +386,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                     // (the offset in the page is 0 unless pages are longer than the tile)
                     const int y = (int)(clamp_page(id) * p.block_size) + (t - pg * p.block_size);
                     const uint32_t bytes = (uint32_t)min(boxes, (last_page - pg + 1) * KB) * (uint32_t)(box_rows * 128);
-                    if (use > 0) wait_bar(empty + stage * 8, (use - 1) & 1);
+                    if (use > 0) wait_together(empty + stage * 8, (use - 1) & 1);
                     if (!alive) break;
                     const uint32_t landed = full + ((MODE == 1 ? (j & 1) * stages : 0) + stage) * 8;
                     if (lane == 0) mbar_arrive_tx(landed, bytes);
@@ -388,7 +396,7 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                     __syncwarp();
                     if (lw == 1 && j == 0 && piece > 0) {
                         // (the rings have room for that tile whatever becomes of this piece's queries)
-                        wait_bar(q_empty, (piece - 1) & 1);
+                        wait_together(q_empty, (piece - 1) & 1);
                         if (!alive) break;
                         load_q();
                     }
@@ -402,7 +410,8 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                 // without this piece's progress) are asked for ahead of them.
                 const int q_after = n > 1 ? 1 : 0;
                 auto load_q = [&]() {                            // a quarter of the rows; rows behind the last are zeros
-                    if (piece >= 1) wait_bar(q_empty, (piece - 1) & 1);
+                    if (piece >= 1) wait_together(q_empty, (piece - 1) & 1);
+                    if (!alive) return;
                     const char* qb = static_cast<const char*>(p.q) + ((size_t)b * p.tokens * p.q_heads + kvh * p.group) * D * 2 + ld_c * 16;
                     for (int x = 0; x < tiles_live; ++x) {
                         int r = lw * (BM / 4) + ld_row0;
@@ -430,7 +439,8 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                     const int pos = t + lw * WR + lane;
                     const uint32_t mine = (uint32_t)(clamp_page(id) * p.block_size + (pos - page_of(pos) * p.block_size));   // below 2^32: the launcher checks it
                     if (j + 1 < n) id = ask(t + BN);
-                    if (J >= NSK) wait_bar(k_empty + stage_k * 8, ((J / NSK) - 1) & 1);
+                    if (J >= NSK) wait_together(k_empty + stage_k * 8, ((J / NSK) - 1) & 1);
+                    if (!alive) break;
 #pragma unroll 8
                     for (int i = 0; i < WR / RPI; ++i) {
                         const int r = i * RPI + ld_row0, row = lw * WR + r;
@@ -440,7 +450,8 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                                       valid ? 16 : 0, 0);
                     }
                     tc::cp_async_arrive(k_full + stage_k * 8);
-                    if (J >= NSV) wait_bar(v_empty + stage_v * 8, ((J / NSV) - 1) & 1);
+                    if (J >= NSV) wait_together(v_empty + stage_v * 8, ((J / NSV) - 1) & 1);
+                    if (!alive) break;
 #pragma unroll 8
                     for (int i = 0; i < WR / RPI; ++i) {
                         const int r = i * RPI + ld_row0, row = lw * WR + r;
