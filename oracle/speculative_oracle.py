@@ -99,3 +99,50 @@ def copy_pages(cache, src, dst):
         if 0 <= i < cache.shape[0] and 0 <= j < cache.shape[0]:
             new[j] = cache[i]
     return new
+
+
+def norm_rope_rows(x, weight, cos_sin, positions, *, eps, interleaved):
+    """`norm_rope` for many tokens at once."""
+    x = x.double()
+    y = x if weight is None else x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) * weight.double()
+    r = cos_sin.shape[1]
+    pos = positions.long()
+    live = ((pos >= 0) & (pos < cos_sin.shape[0]))[:, :, None, None]
+    angles = cos_sin.double()[pos.clamp(0, cos_sin.shape[0] - 1)][:, :, None]
+    c, s = angles[..., : r // 2], angles[..., r // 2:]
+    lo, hi = (slice(0, r, 2), slice(1, r, 2)) if interleaved else (slice(0, r // 2), slice(r // 2, r))
+    out = y.clone()
+    out[..., lo] = y[..., lo] * c - y[..., hi] * s
+    out[..., hi] = y[..., hi] * c + y[..., lo] * s
+    return torch.where(live, out, torch.zeros_like(out)), y.abs().amax(-1, keepdim=True)
+
+
+def tree_decode_rows(q, k_cache, v_cache, table, lens, mask, drafts, scale=None):
+    """`tree_decode` with all rows of a sequence and kv head at once."""
+    b_, t_, hq, d = q.shape
+    hkv, bs = k_cache.shape[2], k_cache.shape[1]
+    g = hq // hkv
+    scale = 1.0 / math.sqrt(d) if scale is None else scale
+    out = torch.zeros(q.shape, dtype=torch.float64)
+    mag = torch.zeros(q.shape, dtype=torch.float64)
+    for b in range(b_):
+        n_keys = min(max(int(lens[b]), 0), table.shape[1] * bs)
+        n = t_ if drafts is None else min(max(int(drafts[b]), 0), t_)
+        if n_keys == 0 or n == 0:
+            continue
+        pages = table[b, : (n_keys + bs - 1) // bs].long()
+        k = k_cache[pages].flatten(0, 1)[:n_keys].double().transpose(0, 1)      # [hkv, keys, d]
+        v = v_cache[pages].flatten(0, 1)[:n_keys].double().transpose(0, 1)
+        number = torch.arange(n_keys) - (n_keys - n)                            # of the drafted token
+        if mask is None:
+            seen = number[None] <= torch.arange(n)[:, None]
+        else:
+            seen = (number[None] < 0) | ((mask[b, :n, None] >> number.clamp(0, 63)[None]) & 1).bool()
+        rows = q[b, :n].double().view(n, hkv, g, d).permute(1, 2, 0, 3)         # [hkv, g, n, d]
+        s = torch.einsum("hgnd,hkd->hgnk", rows, k) * scale
+        s = s.masked_fill(~seen, -math.inf)
+        any_seen = seen.any(1)[:, None]
+        p = torch.where(any_seen, torch.softmax(s, -1), torch.zeros_like(s))
+        out[b, :n] = torch.einsum("hgnk,hkd->nhgd", p, v).reshape(n, hq, d)
+        mag[b, :n] = torch.einsum("hgnk,hkd->nhgd", p, v.abs()).reshape(n, hq, d)
+    return out, mag

@@ -989,3 +989,211 @@ def test_norm_rope_in_place_refuses_a_tensor_that_is_queries_and_keys():
             attn.qk_norm_rope_append(x, k, v, None, None, cs, pos, kc, vc, table, out=x)
     a, b = attn.qk_norm_rope(x, x, None, None, cs, pos)         # as two inputs it is as good as any other
     assert a.data_ptr() != b.data_ptr()
+
+
+# --------------------------------------------------------------------------- paths that take more rows, pieces or tokens
+def test_the_oracles_for_many_rows_are_the_oracles():
+    case = tree_case([0, 1, 9, 40, 17], 6, 6, 2, 16, 4, torch.float32, seed=3, drafts=[6, 6, 0, 5, 99], masks="random")
+    for masks in (case[5], None):
+        args = (*case[:5], masks, case[6])
+        for a, b in zip(ref.tree_decode(*args), ref.tree_decode_rows(*args)):
+            torch.testing.assert_close(a, b, atol=1e-12, rtol=1e-12)
+    gen = torch.Generator().manual_seed(0)
+    x, w = torch.randn(2, 5, 3, 12, generator=gen), torch.randn(12, generator=gen)
+    pos = torch.tensor([[0, 5, -1, 9, 3], [10, 2, 1, 1, 4]], dtype=torch.int32)
+    for interleaved in (False, True):
+        for weight in (w, None):
+            args = (x, weight, rope_table(10, 8), pos)
+            for a, b in zip(ref.norm_rope(*args, eps=1e-5, interleaved=interleaved),
+                            ref.norm_rope_rows(*args, eps=1e-5, interleaved=interleaved)):
+                torch.testing.assert_close(a, b, atol=1e-12, rtol=1e-12)
+
+
+def check_tree_rows(got, case):
+    """`check_tree` with the oracle for many rows."""
+    q, k, v, table, lens, mask, dl = case
+    want, mag = ref.tree_decode_rows(q, k, v, table, lens, mask, dl)
+    d, dtype = q.shape[-1], q.dtype
+    h = half_step(dtype)
+    size = float(q.double().norm(dim=-1).max()) * float(k.double().norm(dim=-1).max()) / math.sqrt(d)
+    fp32 = 2 * d * 2.0**-23 * size + 2.0**-20 + int(lens.max()) * 2.0**-23
+    p_round = 0.0 if dtype == torch.float32 else h
+    got = got.cpu().double()
+    assert ((got - want).abs() <= h * want.abs() + (p_round + fp32) * mag + smallest(dtype)).all()
+    for b in range(q.shape[0]):
+        assert float((got[b] - want[b]).norm()) <= (h + fp32) * float(want[b].norm())
+
+
+ROWS = [(8, 12), (16, 14), (40, 10), (60, 10)]          # drafted tokens, heads of two kv heads: 48, 112, 200, 300 rows each
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bs", [16, 1, 24])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t,hq", ROWS)
+def test_tree_many_rows_and_hidden_infinities(dtype, t, hq, d, bs):
+    """Several softmax warps, and two chains with a query tile each, look through the same drafted values."""
+    lengths = [t, t + 20, 140, 256 + t // 2, 420]
+    q, k, v, table, lens, _, _ = case = tree_case(lengths, t, hq, 2, d, bs, dtype, seed=t + d)
+    shown = 0b1010 | 1 << (t - 2)
+    mask = torch.full((len(lengths), t), shown if t < 64 else shown - (1 << 64), dtype=torch.int64)
+    mask[0, 2] = 0                                              # no prefix either: nothing
+    mask[2, t - 1] = 0                                          # the prefix alone
+    clean = (q, k, v, table, lens, mask, None)
+    bad = [float("nan"), float("inf"), float("-inf")]
+    k, v = k.clone(), v.clone()
+    for b, n in enumerate(lengths):
+        for j in range(t):
+            if shown >> j & 1:
+                continue
+            page, line = int(table[b, (n - t + j) // bs]), (n - t + j) % bs
+            k[page, line], v[page, line] = bad[j % 3], bad[(j + b) % 3]
+        for pos in range(n, (n + bs - 1) // bs * bs):           # behind the end
+            page = int(table[b, pos // bs])
+            k[page, pos % bs], v[page, pos % bs] = bad[pos % 3], bad[(pos + 1) % 3]
+    dq, dk, dv, dt, dl, dm, _ = on_gpu(q, k, v, table, lens, mask, None)
+    got = attn.gqa_tree_decode(dq, dk, dv, dt, dl, dm)
+    check_tree_rows(got, clean)
+    assert torch.count_nonzero(got[0, 2]) == 0
+    assert torch.equal(got, attn.gqa_tree_decode(dq, *on_gpu(clean[1], clean[2]), dt, dl, dm))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bs", [16, 1, 24])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("t,hq", ROWS)
+def test_tree_many_rows_and_infinities_that_some_see(dtype, t, hq, d, bs):
+    """Drafted tokens on both sides of a tile's border, infinite in a column each of one kv head."""
+    lengths = [t, 128 + t // 2, 256 + t - 2, 390]
+    q, k, v, table, lens, mask, _ = tree_case(lengths, t, hq, 2, d, bs, dtype, seed=t * d)
+    v = v.clone()
+    want = torch.zeros(q.shape, dtype=torch.bool)
+    for j, col in ((0, 3), (2, d - 1), (t // 2, d // 2 - 1), (t - 2, d // 2), (t - 1, 0)):
+        seen = ((mask >> j) & 1) == 1
+        want[:, :, hq // 2:, col] |= seen[:, :, None]
+        for b, n in enumerate(lengths):
+            v[int(table[b, (n - t + j) // bs]), (n - t + j) % bs, 1, col] = float("inf")
+    got = attn.gqa_tree_decode(*on_gpu(q, k, v, table, lens, mask)).cpu()
+    assert torch.equal(torch.isinf(got) & (got > 0), want)
+    assert torch.isfinite(got[~want]).all()
+    zero = v.clone()
+    zero[torch.isinf(zero)] = 0                                 # what is finite must not have changed by it
+    clean = attn.gqa_tree_decode(*on_gpu(q, k, zero, table, lens, mask)).cpu()
+    assert torch.equal(got[~want], clean[~want])
+
+
+@gpu
+@pytest.mark.parametrize("kernel", ["auto", "simt"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,hq,hkv,d", [(10, 20, 2, 256), (30, 20, 2, 256), (64, 8, 1, 200), (7, 80, 2, 256), (64, 64, 4, 128),
+                                        (64, 32, 4, 64), (64, 32, 2, 80)])
+def test_tree_wide_heads_and_several_blocks_of_rows(dtype, kernel, t, hq, hkv, d):
+    """More rows than a query tile at D above 128, and more than two query tiles below."""
+    case = tree_case([t, 200, 129, 700], t, hq, hkv, d, 16, dtype, seed=d + t, drafts=[t, t - 1, 0, t])
+    dc = on_gpu(*case)
+    check_tree_rows(attn.gqa_tree_decode(*dc[:6], draft_lens=dc[6], kernel=kernel), case)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("batch,d,bs", [(400, 128, 16), (800, 64, 16), (250, 256, 16), (300, 128, 24), (1000, 37, 16)])
+def test_tree_more_sequences_than_a_cta_has_threads(dtype, batch, d, bs):
+    """The lengths are added up in several rounds."""
+    gen = torch.Generator().manual_seed(batch)
+    lengths = [int(x) for x in torch.randint(0, 150, (batch,), generator=gen)]
+    lengths[0], lengths[-1], lengths[batch // 2] = 0, 0, 600
+    case = tree_case(lengths, 3, 4, 2, d, bs, dtype, seed=batch)
+    check_tree_rows(attn.gqa_tree_decode(*on_gpu(*case[:6])), case)
+
+
+@gpu
+@pytest.mark.parametrize("kernel", ["auto", "simt"])
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64), (torch.bfloat16, 256), (torch.float32, 128),
+                                     (torch.float32, 37), (torch.float16, 66)])
+@pytest.mark.parametrize("t,hq,batch,tiles", [(1, 1, 1, 79), (3, 4, 1, 140), (2, 1, 2, 31), (2, 4, 2, 32), (2, 1, 2, 33), (5, 1, 2, 64),
+                                              (2, 2, 2, 65)])
+@pytest.mark.parametrize("trend", [6.0, -6.0])
+def test_tree_sequences_cut_into_many_pieces(dtype, d, kernel, t, hq, batch, tiles, trend):
+    """One kv head and a run a tile: the merge joins 32 pieces at a time and carries the rest on.  The scores rise
+    (or fall) along the sequence, so that the maxima of the pieces differ and early (late) ones weigh little."""
+    tile = 64 if kernel == "simt" or dtype == torch.float32 or d % 8 else 128
+    lengths = [tiles * tile - 3, tiles * tile][:batch]
+    q, k, v, table, lens, mask, _ = tree_case(lengths, t, hq, 1, d, 16, dtype, seed=tiles)
+    q[..., 0] = 2.0
+    for b, n in enumerate(lengths):
+        pages = table[b, : (n + 15) // 16].long()
+        ramp = torch.linspace(-0.5, 0.5, 16 * len(pages)).view(-1, 16, 1) * trend * math.sqrt(d) / 2
+        k[pages, ..., 0] = ramp.to(dtype)
+    case = (q, k, v, table, lens, mask, None)
+    dc = on_gpu(*case[:6])
+    got = attn.gqa_tree_decode(*dc, kernel=kernel)
+    check_tree_rows(got, case)
+    assert torch.equal(got, attn.gqa_tree_decode(*dc, kernel=kernel))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,rot,hq,hkv", [(64, 64, 7, 3), (128, 128, 6, 1), (80, 48, 8, 4), (256, 256, 7, 3), (96, 96, 5, 2),
+                                          (128, 64, 9, 3)])
+def test_norm_rope_of_many_tokens(dtype, interleaved, d, rot, hq, hkv):
+    """Enough rows for four heads per group of lanes: heads that are no multiple of four, padding, slices of one
+    projection's output, in place; the same bits as the same tokens in small calls, which take a head at a time."""
+    gen = torch.Generator().manual_seed(d + hq)
+    lanes = 8 if d <= 64 else 16 if d <= 128 else 32             # of a group
+    b, heads = 2, hq + 2 * hkv
+    t = 4 * 148 * 1024 // (b * (hq + hkv) * lanes) + 3           # a little more than four heads a group begin at
+    qkv = torch.randn(b, t, heads, d, generator=gen).to(dtype)
+    w = (1 + 0.2 * torch.randn(2, d, generator=gen)).to(dtype)
+    cs = rope_table(300, rot)
+    pos = torch.randint(0, 300, (b, t), generator=gen, dtype=torch.int32)
+    pos[0, 5], pos[1, t - 1], pos[1, 0] = -1, 300, 2**31 - 1
+    dqkv, dw, dcs, dp = on_gpu(qkv, w, cs, pos)
+    q, k, v = dqkv.split([hq, hkv, hkv], 2)
+    a, c = attn.qk_norm_rope(q, k, dw[0], dw[1], dcs, dp, interleaved=interleaved)
+    for got, x, weight in ((a, qkv[:, :, :hq], w[0]), (c, qkv[:, :, hq:hq + hkv], w[1])):
+        want, m = ref.norm_rope_rows(x, weight, cs, pos, eps=1e-6, interleaved=interleaved)
+        assert ((got.cpu().double() - want).abs() <= half_step(dtype) * want.abs() + 2.1e-6 * m + smallest(dtype)).all()
+    for lo in range(0, t, 97):
+        part = slice(lo, min(t, lo + 97))
+        x, y = attn.qk_norm_rope(q[:, part], k[:, part], dw[0], dw[1], dcs, dp[:, part].contiguous(), interleaved=interleaved)
+        assert torch.equal(x, a[:, part]) and torch.equal(y, c[:, part])
+    # into the cache: every other token's slot is out of range, one page is outside the pool
+    bs, pages = 16, (t + 15) // 16
+    kc, vc = torch.randn(2, b * pages, bs, hkv, d, generator=gen).to(dtype).to(DEV)
+    want_k, want_v = kc.cpu(), vc.cpu()
+    table = torch.randperm(b * pages, generator=gen).view(b, pages).to(torch.int32)
+    table[1, 1] = -1
+    slots = torch.arange(t, dtype=torch.int32).repeat(b, 1)
+    slots[:, 1::2] = torch.tensor([[-1], [pages * bs]], dtype=torch.int32)
+    out = attn.qk_norm_rope_append(q, k, v, dw[0], dw[1], dcs, dp, kc, vc, table.to(DEV), slots=slots.to(DEV),
+                                   interleaved=interleaved)
+    assert torch.equal(out, a)
+    live = (pos >= 0) & (pos < 300)
+    ref.write_rows(want_k, c.cpu(), table, slots, live)
+    ref.write_rows(want_v, qkv[:, :, hq + hkv:], table, slots, live)
+    assert torch.equal(kc.cpu(), want_k) and torch.equal(vc.cpu(), want_v)
+    # in place, and without a norm
+    q, k = q.contiguous(), k.contiguous()
+    plain = attn.qk_norm_rope(q, k, None, None, dcs, dp, interleaved=interleaved)
+    want, m = ref.norm_rope_rows(qkv[:, :, :hq], None, cs, pos, eps=1e-6, interleaved=interleaved)
+    assert ((plain[0].cpu().double() - want).abs() <= half_step(dtype) * want.abs() + 2.1e-6 * m + smallest(dtype)).all()
+    attn.qk_norm_rope(q, k, dw[0], dw[1], dcs, dp, interleaved=interleaved, q_out=q, k_out=k)
+    assert torch.equal(q, a) and torch.equal(k, c)
+
+
+@gpu
+@pytest.mark.parametrize("kernel", ["auto", "simt"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bs", [16, 24])
+def test_tree_lengths_outside_the_table_are_clamped(dtype, kernel, bs):
+    """Negative lengths are empty sequences, longer ones than the table holds end with it, drafted tokens last."""
+    q, k, v, table, lens, mask, _ = tree_case([240, 240, 240, 100], 5, 6, 2, 64, bs, dtype, seed=1)
+    cap = table.shape[1] * bs
+    wild = torch.tensor([2**31 - 1, -7, cap + 1, -2**31], dtype=torch.int32)
+    case = (q, k, v, table, wild, mask, None)
+    got = attn.gqa_tree_decode(*on_gpu(*case[:6]), kernel=kernel)
+    check_tree_rows(got, (q, k, v, table, wild.clamp(0, cap), mask, None))
+    assert torch.count_nonzero(got[1]) == 0 and torch.count_nonzero(got[3]) == 0
