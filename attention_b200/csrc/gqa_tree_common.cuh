@@ -185,7 +185,9 @@ __device__ __forceinline__ long long tree_part_row(const TreeParams& p, int slot
 // that a long sequence's many pieces cost a few round trips to memory and not some each; then the warp
 // adds the pieces' rows, kTreeMergeRows rows by four pieces at a time.
 // Its reads are the partials, 4 D + 8 bytes a row and piece, mostly still in L2; bound by round trips: 6 to
-// 8 us alone with 2 pieces a row (144 runs), 4 of them behind the attention kernel's last CTAs.
+// 8 us alone with 2 pieces a row (144 runs), 4 of them behind the attention kernel's last CTAs; 25 us with 18
+// pieces of 2048 rows.  The pieces of a row are one warp's work, so that a single long sequence with one kv head
+// pays most: 148 pieces of 8 rows (32 k keys) take 47 us, of 64 rows 57, as long as their attention (44 and 50).
 // NV4 > 0: D is a multiple of 4 and at most 128 NV4, a lane owns columns 4 lane .. 4 lane + 3 (and + 128).
 // ---------------------------------------------------------------------------
 constexpr int kTreeMergeWarps = 8;

@@ -8,9 +8,9 @@
 // the probabilities cross a warp, never the CTA, and the running maxima and sums stay in registers.
 // A warp reads a K element once for two rows (RB = 8) to eight (RB = 32): the shared-memory reads,
 // not the arithmetic, are what RB amortises, so few rows take the small block and many the large.
-// They are what bounds it: fp32, D 128, batch 16 of 1 to 4 k keys, 8 tokens 280 us (19 TFLOP/s), 32 tokens
-// 1010 us; 4 tokens at batch 64 786 us (1.7 TB/s).  A batch of four short sequences takes 28 us, most of
-// it trips to memory (lengths, page ids, keys) and the merge.
+// They bound many rows, and with few the loads, which nothing of the CTA overlaps: fp32, D 128, batch 16 of 1 to
+// 4 k keys, 8 tokens 280 us (19 TFLOP/s), 32 tokens 1010 us (21); 4 tokens at batch 64 785 us (1.7 TB/s).  A batch of
+// four short sequences takes 28 to 35 us, most of it trips to memory (lengths, page ids, keys) and the merge.
 #pragma once
 
 #include <type_traits>

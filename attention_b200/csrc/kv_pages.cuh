@@ -35,9 +35,11 @@ __device__ __forceinline__ long long page_row_offset(const CompactParams& p, int
 // a barrier, all writes.  Slices are columns that no other CTA touches, so whatever the list
 // holds (a permutation, the same source twice, a source that is another entry's destination),
 // every entry gets the row as it was before the call.
-// What bounds it: dependent trips to memory (positions, page ids, rows, writes); a few
-// rows cost a launch and those trips, 4 to 5 us for 8 sequences x 5 rows of 2 KB, 7 us for 256 x 16 (2.5 TB/s).  A thread
-// holds up to eight granules so that its reads are all under way before the barrier.
+// What bounds it: for a few rows a launch and dependent trips to memory (positions, page ids, rows, writes), 4 to 5 us
+// for 8 sequences x 5 rows of 2 KB; for 256 x 16 rows, 6.6 to 8 us (2.2 to 2.7 TB/s), its own index arithmetic as well:
+// two 64-bit divisions an entry and a division by the run-time width a granule keep 45 % of the issue slots and
+// 23 % of the special-function pipe busy.  A thread holds up to eight granules so that its reads are all under
+// way before the barrier.
 template <typename UNIT>
 __global__ void __launch_bounds__(kCompactThreads) kv_compact_kernel(const CompactParams p) {
     __shared__ long long s_from[kCompactMaxRows], s_to[kCompactMaxRows];

@@ -95,6 +95,8 @@ template <typename T> __device__ __forceinline__ float rope_weight(const RopePar
 // Every head_dim in [1, 256], every alignment and stride: one warp per head row, elements lane,
 // lane + 32, ...  A lane also reads the partners of its elements (first-level cache hits), and
 // every read of the row precedes its writes, so the output may be the input.
+// Bound by issue, an element at a time: 16384 tokens x 72 heads of 100 16-bit elements take 840 us (0.57 TB/s),
+// of 128 with 28 rotated 685, where the kernel below takes 117.
 constexpr int kRopeWarps = 4;
 template <typename T>
 __global__ void __launch_bounds__(kRopeWarps * 32) qk_norm_rope_any_kernel(const RopeParams p) {
