@@ -65,10 +65,11 @@
 // Precision: scores and sums in fp32, O in fp32, P rounded to the element type for the products.  In bf16
 // that is a relative error of half a step of each probability.  fp16 has that only down to 2^-14, and a key
 // that is 2^-25 of the row's reference would be nothing: many such keys below one whose value is small are
-// the result.  So fp16 probabilities are lifted by 2^kTreeLift, P = 2^(s - reference + lift), and the
-// reference follows the maximum more closely (kTreeSlack) to stay in range, P <= 2^15: half a step down to
-// 2^-25 of the largest, below that an absolute error of up to 2^-36 of it a key.  The lift is in P's sums as
-// well and cancels in their quotient; maxima that leave the chain are without it.  (Batch of 64 sequences of
+// the result.  So the reference of fp16 rows is set tree_lift = 11 below the maximum and follows it more
+// closely (kTreeSlack): P = 2^(s - reference) <= 2^15, half a step down to 2^-25 of the largest, below that an
+// absolute error of up to 2^-36 of it a key.  P's sums are over the same reference, so it cancels in their
+// quotient.  Scores beyond 2^20, which fp32 holds to an eighth of a unit and less, have a smaller lift: the
+// maximum, the product behind it and the reference are each off by up to half a step (4 at 2^26).  (Batch of 64 sequences of
 // 1 to 4 k keys, 16 tokens: no lift and a slack of 8, 128 us; 11 and 4, 130 to 135; 13 and 2, whose sums move
 // much more often, 147.  D 256, 64 tokens, batch 16: 130, 131 and 156.)
 #pragma once
@@ -90,8 +91,12 @@ static __device__ int g_tree_tc_status;
 constexpr int kTreeBM = 128;            // rows of a query tile
 constexpr int kTreeTmemCols = 512;
 
-// log2 of what P is multiplied by, and how far a maximum may lie above its row's reference
-template <typename T> constexpr float kTreeLift = std::is_same<T, __half>::value ? 11.f : 0.f;
+// How far (log2 units) a row's reference is set below its maximum `mx`, and how much higher the maximum may then
+// rise before it is set again.
+template <typename T> __device__ __forceinline__ float tree_lift(float mx) {
+    if constexpr (std::is_same<T, __half>::value) return fabsf(mx) < 1048576.f ? 11.f : 7.f;
+    else return 0.f;
+}
 template <typename T> constexpr float kTreeSlack = std::is_same<T, __half>::value ? 4.f : kRescaleSlack;
 
 template <int DP, int MODE> struct TreeTcGeom {
@@ -599,15 +604,16 @@ gqa_tree_tc_kernel(const TreeParams p, const __grid_constant__ CUtensorMap map_q
                         a1 = tc::max3(a1, sc[HN - 2], sc[HN - 1]);
                         mx = fmaxf(tc::max3(a0, a1, a2), a3) * p.scale_log2;
                     }
-                    const bool need = live && mx > m_run + kTreeSlack<T>;
+                    const float lift = tree_lift<T>(mx);
+                    const bool need = live && mx - m_run > lift + kTreeSlack<T>;
                     float alpha = 1.f;
                     if (need) {
-                        const float mn = fmaxf(m_run, mx);
+                        const float mn = mx - lift;
                         alpha = m_run == -INFINITY ? 0.f : fast_exp2(m_run - mn);
                         m_run = mn;
                         l_run *= alpha;
                     }
-                    const float nref = m_run == -INFINITY ? 0.f : kTreeLift<T> - m_run;
+                    const float nref = m_run == -INFINITY ? 0.f : -m_run;
 #pragma unroll
                     for (int c = 0; c < HN; c += 2) tc::fma2(sc[c], sc[c + 1], sc[c], sc[c + 1], p.scale_log2, nref);
 #pragma unroll

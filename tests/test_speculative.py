@@ -378,6 +378,31 @@ def test_tree_probabilities_far_below_a_dominating_key(dtype, kernel, nats, t, h
 
 
 @gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", [0.0, 10.0, 1500.0, 3000.0, 6000.0])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("t,hq,d,bs", [(4, 4, 64, 16), (40, 8, 64, 16), (16, 8, 128, 16), (4, 4, 256, 16), (4, 4, 64, 24)])
+def test_tree_probabilities_stay_in_range_whatever_the_scores(dtype, size, sign, t, hq, d, bs):
+    """Scores of up to 2^26 that differ by a few units (a step of fp32 is 4 there), and a value that is the same for
+    every key: the weighted mean is that value.  What the weights are does not matter, but a probability
+    must not overflow its type.  Their rounding is off by h(t), below fp16's normal numbers by 2^-25 where the largest
+    is 4 at least (the reference may be off by a step): 2^-27 a key."""
+    lengths = [600, 77, 300]
+    gen = torch.Generator().manual_seed(7)
+    q, k, v, table, lens, mask, _ = tree_case(lengths, t, hq, 2, d, bs, dtype, seed=t)
+    q, k = 0 * q, 0 * k
+    q[..., 0], k[..., 0] = 60000.0, sign * size * math.sqrt(d) / 8.0
+    q[..., 1] = 8.0
+    k[..., 1] = (torch.rand(k.shape[:-1], generator=gen) * 20).to(dtype)
+    v = v[:1, :1].expand(v.shape).contiguous()
+    got = attn.gqa_tree_decode(*on_gpu(q, k, v, table, lens, mask)).cpu().double()
+    want = v[0, 0].double().repeat_interleave(hq // 2, 0).expand(got.shape)
+    p_round = 0.0 if dtype == torch.float32 else half_step(dtype)
+    rel = half_step(dtype) + p_round + max(lengths) * 2.0**-23 + 2.0**-20 + max(lengths) * 2.0**-27
+    assert ((got - want).abs() <= rel * want.abs() + smallest(dtype)).all()
+
+
+@gpu
 @pytest.mark.parametrize("kernel", ["auto", "simt"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("shape", [(300, 3, 4, 2), (2, 7, 64, 64), (1, 64, 16, 2), (5, 20, 40, 8), (1, 1, 1, 1)])
